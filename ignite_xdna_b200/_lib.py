@@ -21,10 +21,11 @@ IXB_ERR_DEVICE = -4
 IXB_ERR_CAPACITY = -6
 IXB_ERR_UNSUPPORTED = -5
 MAX_SEGS = 4
-API_VERSION = 9
+API_VERSION = 10
 MAX_EXTRA_SLOTS = 3
 MODE_WINDOW, MODE_GATHER, MODE_STEM, MODE_IM2COL = 0, 1, 2, 3
 OUT2_NONE, OUT2_UP2, OUT2_S2D, OUT2_S2D_ONLY = 0, 1, 2, 3
+BF16, F16, F32 = 0, 1, 2
 IN_DEVICE, OUT_DEVICE, ASYNC, NO_GRAPH, IN_STORE = 1, 2, 4, 8, 16
 OP_CONV, OP_POOL = 0, 1
 OP_WITH_PREV = 0x100     # a conv that runs concurrently with the op(s) before it (branch group)
@@ -117,6 +118,15 @@ _SIGS = {
                                 C.c_void_p]),
     "ixb_w4a8_gemv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "ixb_u8i4_gemm_i32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "ixb_fp8_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                   C.c_void_p, C.c_int64, C.c_void_p]),
+    "ixb_rmsnorm_quant": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                    C.c_int, C.c_float, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_int64, C.c_void_p]),
+    "ixb_fp8_linear": (C.c_int, [C.c_void_p, C.c_int64] * 4 + [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                                               C.c_void_p]),
+    "ixb_fp8_linear_swiglu": (C.c_int, [C.c_void_p, C.c_int64] * 8 + [C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "ixb_fp8_plan_info": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32), C.c_int]),
     "ixb_decode_yolo": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int32, C.c_void_p,
                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ixb_decode_yolo_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int32,

@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <chrono>
 #include <cmath>
 #include <cstdio>
@@ -25,6 +26,7 @@
 #include "../../include/ixb200.h"
 #include "ixb_conv.cuh"
 #include "ixb_decode.cuh"
+#include "ixb_fp8.cuh"
 #include "ixb_gemm.cuh"
 #include "ixb_misc.cuh"
 #include "ixb_w4a8.cuh"
@@ -997,6 +999,198 @@ int check_w4a8_shape(int N, int K) {
   if (N < 16 || N % 16 || K < kW4Group || K % kW4Group || K > 65536)
     return fail(IXB_ERR_INVALID, "W4A8 needs N a multiple of 16 and K a multiple of 128, at most 65536");
   return 0;
+}
+
+// ---------------------------------------------------------------- fp8 linears
+constexpr int kFp8Align = 16;  // bytes: pointers and row strides of what TMA or vector loads touch
+
+bool aligned_rows(const void* ptr, long long ld_bytes) { return aligned16(ptr) && ld_bytes % kFp8Align == 0; }
+int type_size(int type) { return type == IXB_F32 ? 4 : 2; }
+bool known_type(int type) { return type == IXB_BF16 || type == IXB_F16 || type == IXB_F32; }
+
+// Tensor map of an e4m3 [rows][K] matrix with rows ld bytes apart: boxes of 128 bytes of K by
+// box_rows rows, 128-byte swizzled; rows past the end and K past its end read as zero.
+int encode_rows(CUtensorMap* map, const void* base, long long rows, int K, long long ld, int box_rows, std::string& err) {
+  auto enc = tiled_encoder(err);
+  if (!enc) return -1;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    err = "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+    return -1;
+  }
+  return 0;
+}
+
+struct Fp8Launch {
+  Fp8Params p;
+  int mt, grid, smem;
+};
+
+// Tile (MT blocks of 128 weight rows x bn tokens), split of K over a cluster, pipeline depth and
+// grid for M tokens x N outputs x K: the choice with the least estimated SM cycles.
+int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
+  Fp8Params& p = L.p;
+  memset(&p, 0, sizeof p);
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.kblocks = (K + 127) / 128;
+  const int sms = sm_count();
+  double best = 1e300;
+  const int m16 = std::min(256, round_up(M, 16));
+  const int nblk = (N + 127) / 128;
+  for (int mt : {1, 2}) {
+    if (mode == FP8_SWIGLU ? mt == 1 : (mt == 2 && nblk == 1)) continue;
+    const long long n_tiles = mode == FP8_SWIGLU ? nblk : (nblk + mt - 1) / mt;
+    for (int bn = 16; bn <= m16; bn += 16) {
+      const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
+      if (mt * bn + sf_cols > 512) break;
+      const long long tiles = n_tiles * ((M + bn - 1) / bn);
+      const int stage = mt * kGemmABlock + bn * 128;
+      for (int split : {1, 2, 4, 8}) {
+        const int kbs = (p.kblocks + split - 1) / split;
+        if (split > 1 && ((long long)(split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms ||
+                          mt * bn * 512 > std::min(kFp8MaxStages, 180 * 1024 / stage) * stage))
+          break;
+        const long long waves = (tiles * split + sms - 1) / sms;
+        const bool two = split == 1 && waves > 1 && 2 * mt * bn + sf_cols <= 512;
+        const double mma = mt * std::max(2.0 * bn, 128.0), load = stage / 45.0;
+        const double epi = 8.0 * mt * bn / (split > 1 ? 2 : 1) + (split > 1 ? 1500.0 : 0.0);
+        const double cost = waves * (kbs * std::max(mma, load) + (two ? 0.0 : epi)) + (two ? epi : 0.0);
+        if (cost < best) {
+          best = cost;
+          L.mt = mt;
+          p.bn = bn;
+          p.split = split;
+          p.kb_split = kbs;
+          p.nacc = two ? 2 : 1;
+        }
+      }
+    }
+  }
+  const int mt = L.mt;
+  p.n_tiles = mode == FP8_SWIGLU ? nblk : (nblk + mt - 1) / mt;
+  p.m_tiles = (M + p.bn - 1) / p.bn;
+  const long long tiles = (long long)p.n_tiles * p.m_tiles;
+  if (tiles * p.split > 0x7fffffffLL) {
+    err = "too many tiles";
+    return -1;
+  }
+  L.grid = (int)(p.split > 1 ? tiles * p.split : std::min<long long>(tiles, sms));
+  p.stage_bytes = mt * kGemmABlock + p.bn * 128;
+  const int groups = (p.bn + 127) / 128;
+  const int sf = kSfSlots * (mt + groups) * kSfAtom;
+  const int stg = p.split > 1 ? 0 : 2 * (mode == FP8_SWIGLU ? 2 : 1) * kFp8Chunk * 128 * 4;
+  // two CTAs per SM when a split grid has more CTAs than SMs
+  const int limit = L.grid > sms ? kSmemLimit / 2 - 1024 : kSmemLimit;
+  const int red = p.split > 1 ? mt * p.bn * 512 : 0;
+  p.stages = std::min(kFp8MaxStages, (limit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
+  if (p.split > 1 || p.stages * p.stage_bytes < red || p.stages < 2) {
+    p.stages = std::min(kFp8MaxStages, (kSmemLimit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
+    p.stages = std::max(std::min(p.stages, p.kb_split), (red + p.stage_bytes - 1) / p.stage_bytes);
+  }
+  p.stages = std::max(p.stages, 1);
+  p.sf_off = p.stages * p.stage_bytes;
+  p.stg_off = p.sf_off + sf;
+  p.bar_off = p.stg_off + stg;
+  L.smem = 1024 + p.bar_off + kFp8BarBytes;
+  p.acc_cols = mt * p.bn;
+  const int need = p.nacc * p.acc_cols + 2 * 4 * (mt + groups);
+  p.tmem_cols = 32;
+  while (p.tmem_cols < need) p.tmem_cols *= 2;
+  p.idesc = umma_idesc_mxf8(128, p.bn);
+  if (L.smem > kSmemLimit || p.tmem_cols > 512) {
+    err = "no tile fits";
+    return -1;
+  }
+  return 0;
+}
+
+template <int MODE, int MT>
+int launch_fp8(const Fp8Launch& L, cudaStream_t st) {
+  if (int r = ensure_smem_limit(fp8_gemm_kernel<MODE, MT>, kSmemLimit)) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)L.grid);
+  cfg.blockDim = dim3(kFp8Threads);
+  cfg.dynamicSmemBytes = (size_t)L.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (L.p.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)L.p.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  IXB_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<MODE, MT>, L.p));
+  return 0;
+}
+
+// What both products check of an operand: an e4m3 [rows][K] matrix and its scales.
+int check_fp8_operand(const void* v, int64_t ld, const void* s, int64_t lds, int K, const char* what) {
+  if (!v || !s) return fail(IXB_ERR_INVALID, std::string("null ") + what);
+  if (!aligned_rows(v, ld) || ld < K)
+    return fail(IXB_ERR_INVALID, std::string(what) + " must be 16-byte aligned with a row stride of at least K, a multiple of 16");
+  if (lds < (K + 127) / 128) return fail(IXB_ERR_INVALID, std::string(what) + " scales: row stride below ceil(K / 128)");
+  return 0;
+}
+
+int check_fp8_sizes(int M, int N, int K) {
+  if (M < 0 || N < 1 || K < 16 || K % 16 || K > (1 << 20) || N > (1 << 24))
+    return fail(IXB_ERR_INVALID, "fp8 product needs M >= 0, N in [1, 2^24], K a multiple of 16 in [16, 2^20]");
+  return 0;
+}
+
+template <typename T>
+int launch_quantize_fp8(const void* x, int64_t ldx, int M, int K, int block_rows, uint8_t* q, int64_t ldq, uint8_t* scale,
+                        int64_t lds, cudaStream_t st) {
+  const int kb = (K + kQBlock - 1) / kQBlock;
+  const T* xt = static_cast<const T*>(x);
+  if (block_rows == 1) {
+    const long long blocks = (long long)M * kb, per_cta = (kQThreads / 16) * kQUnroll;
+    const unsigned grid = (unsigned)std::min<long long>((blocks + per_cta - 1) / per_cta, 8LL * sm_count());
+    IXB_CUDA(launch_dependent(quantize_rows_kernel<T>, dim3(grid), dim3(kQThreads), 0, st, true, xt, (long long)ldx, K, kb,
+                              blocks, q, (long long)ldq, scale, (long long)lds));
+  } else {
+    IXB_CUDA(launch_dependent(quantize_tiles_kernel<T>, dim3((unsigned)kb, (unsigned)((M + kQBlock - 1) / kQBlock)), dim3(256),
+                              0, st, true, xt, (long long)ldx, M, K, q, (long long)ldq, scale, (long long)lds));
+  }
+  return 0;
+}
+
+template <typename T, typename W>
+int launch_norm(const NormParams& p, cudaStream_t st) {
+  // Threads times V vectors of eight cover the row. Few rows: the most threads, for the shortest
+  // chain of loads. Many: about 256, so that several rows share an SM and hide one another's barriers.
+  const int nvec = p.K / 8, want = p.M > 2 * sm_count() ? 256 : 1024;
+  const unsigned grid = (unsigned)std::min<long long>(p.M, 16LL * sm_count());
+  auto threads = [&](int v) { return (unsigned)round_up((nvec + v - 1) / v, 32); };
+  if (nvec <= want)
+    IXB_CUDA(launch_dependent(norm_quant_kernel<T, W, 1>, dim3(grid), dim3(threads(1)), 0, st, true, p));
+  else if (nvec <= 2 * want)
+    IXB_CUDA(launch_dependent(norm_quant_kernel<T, W, 2>, dim3(grid), dim3(threads(2)), 0, st, true, p));
+  else if (nvec <= 2048)
+    IXB_CUDA(launch_dependent(norm_quant_kernel<T, W, 4>, dim3(grid), dim3(threads(4)), 0, st, true, p));
+  else
+    IXB_CUDA(launch_dependent(norm_quant_kernel<T, W, 8>, dim3(grid), dim3(threads(8)), 0, st, true, p));
+  return 0;
+}
+
+template <typename T>
+int launch_norm_w(const NormParams& p, bool w32, cudaStream_t st) {
+  return w32 ? launch_norm<T, float>(p, st) : launch_norm<T, T>(p, st);
 }
 
 int read_device_error() {
@@ -2191,6 +2385,141 @@ int ixb_gemm_plan_info(int M, int N, int K, int w4a8, int32_t* info, int n) {
                          L.p.tmem_cols, L.p.stage_bytes};
   for (int i = 0; i < n && i < 10; ++i) info[i] = v[i];
   return 0;
+}
+
+int ixb_fp8_quantize(const void* x, int type, int64_t ldx, int M, int K, int block_rows, uint8_t* q, int64_t ldq,
+                     uint8_t* scale, int64_t lds, void* stream) {
+  if (!known_type(type)) return fail(IXB_ERR_INVALID, "unknown value type");
+  if (M < 0 || K < 16 || K % 16 || (block_rows != 1 && block_rows != kQBlock))
+    return fail(IXB_ERR_INVALID, "quantise needs M >= 0, K a multiple of 16, blocks of 1 or 128 rows");
+  if (block_rows == kQBlock && M > 65535 * kQBlock) return fail(IXB_ERR_INVALID, "too many rows for blocks of 128");
+  if (M == 0) return IXB_OK;
+  if (!x || !q || !scale) return fail(IXB_ERR_INVALID, "null argument");
+  if (!aligned_rows(x, ldx * type_size(type)) || !aligned_rows(q, ldq) || ldx < K || ldq < K || lds < (K + kQBlock - 1) / kQBlock)
+    return fail(IXB_ERR_INVALID, "quantise: rows must be 16-byte aligned and at least K apart, scales ceil(K / 128)");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (type == IXB_BF16) return launch_quantize_fp8<__nv_bfloat16>(x, ldx, M, K, block_rows, q, ldq, scale, lds, st);
+  if (type == IXB_F16) return launch_quantize_fp8<__half>(x, ldx, M, K, block_rows, q, ldq, scale, lds, st);
+  return launch_quantize_fp8<float>(x, ldx, M, K, block_rows, q, ldq, scale, lds, st);
+}
+
+int ixb_rmsnorm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int type,
+                      int weight_type, int M, int K, float eps, int position, void* h, int64_t ldh, uint8_t* q, int64_t ldq,
+                      uint8_t* scale, int64_t lds, void* stream) {
+  if (!known_type(type) || (weight_type != type && weight_type != IXB_F32))
+    return fail(IXB_ERR_INVALID, "norm: the weight has the values' type or fp32");
+  if (M < 0 || K < 16 || K % 16 || K > 32768) return fail(IXB_ERR_INVALID, "norm needs M >= 0, K a multiple of 16, at most 32768");
+  if (!(eps >= 0.f) || eps > FLT_MAX) return fail(IXB_ERR_INVALID, "norm: eps must be finite and not negative");
+  if (!scale && (position < -64 || position > 64)) return fail(IXB_ERR_INVALID, "norm: position outside [-64, 64]");
+  if (!residual != !h) return fail(IXB_ERR_INVALID, "norm: a residual comes with its output and the output with a residual");
+  if (M == 0) return IXB_OK;
+  if (!x || !weight || !q) return fail(IXB_ERR_INVALID, "null argument");
+  const int es = type_size(type);
+  if (!aligned_rows(x, ldx * es) || !aligned16(weight) || !aligned_rows(q, ldq) || ldx < K || ldq < K ||
+      (residual && (!aligned_rows(residual, ldr * es) || !aligned_rows(h, ldh * es) || ldr < K || ldh < K)) ||
+      (scale && lds < (K + kQBlock - 1) / kQBlock))
+    return fail(IXB_ERR_INVALID, "norm: rows must be 16-byte aligned and at least K apart, scales ceil(K / 128)");
+  NormParams p = {};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.h = h;
+  p.q = q;
+  p.scale = scale;
+  p.ldx = ldx;
+  p.ldr = ldr;
+  p.ldh = ldh;
+  p.ldq = ldq;
+  p.lds = lds;
+  p.M = M;
+  p.K = K;
+  p.eps = eps;
+  p.unit = scale ? 1.f : ldexpf(1.f, position);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool w32 = weight_type == IXB_F32;
+  if (type == IXB_BF16) return launch_norm_w<__nv_bfloat16>(p, w32, st);
+  if (type == IXB_F16) return launch_norm_w<__half>(p, w32, st);
+  return launch_norm<float, float>(p, st);
+}
+
+int ixb_fp8_linear(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* w, int64_t ldw,
+                   const uint8_t* w_scale, int64_t ldws, void* out, int out_type, int64_t ldo, int M, int N, int K,
+                   void* stream) {
+  if (int r = check_fp8_sizes(M, N, K)) return r;
+  if (!known_type(out_type)) return fail(IXB_ERR_INVALID, "unknown output type");
+  if (M == 0) return IXB_OK;
+  if (int r = check_fp8_operand(x, ldx, x_scale, ldxs, K, "x")) return r;
+  if (int r = check_fp8_operand(w, ldw, w_scale, ldws, K, "w")) return r;
+  if (!out || reinterpret_cast<uintptr_t>(out) % type_size(out_type) || ldo < N)
+    return fail(IXB_ERR_INVALID, "out must be aligned to its type with a row stride of at least N");
+  Fp8Launch L;
+  std::string err;
+  if (plan_fp8(L, M, N, K, FP8_LINEAR, err)) return fail(IXB_ERR_INVALID, err);
+  Fp8Params& p = L.p;
+  if (encode_rows(&p.tx, x, M, K, ldx, p.bn, err) || encode_rows(&p.tw[0], w, N, K, ldw, 128, err))
+    return fail(IXB_ERR_CUDA, err);
+  p.xs = x_scale;
+  p.ldxs = ldxs;
+  p.ws[0] = w_scale;
+  p.ldws[0] = ldws;
+  if (p.m_tiles == 1) {
+    p.w[0] = w;
+    p.ldw[0] = ldw;
+  }
+  p.out = out;
+  p.out_type = out_type;
+  p.ldo = ldo;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return L.mt == 1 ? launch_fp8<FP8_LINEAR, 1>(L, st) : launch_fp8<FP8_LINEAR, 2>(L, st);
+}
+
+int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* gate,
+                          int64_t ldg, const uint8_t* gate_scale, int64_t ldgs, const uint8_t* up, int64_t ldu,
+                          const uint8_t* up_scale, int64_t ldus, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int M,
+                          int N, int K, void* stream) {
+  if (int r = check_fp8_sizes(M, N, K)) return r;
+  if (N % 16) return fail(IXB_ERR_INVALID, "swiglu needs N a multiple of 16");
+  if (M == 0) return IXB_OK;
+  if (int r = check_fp8_operand(x, ldx, x_scale, ldxs, K, "x")) return r;
+  if (int r = check_fp8_operand(gate, ldg, gate_scale, ldgs, K, "gate")) return r;
+  if (int r = check_fp8_operand(up, ldu, up_scale, ldus, K, "up")) return r;
+  if (int r = check_fp8_operand(q, ldq, scale, lds, N, "q")) return r;
+  Fp8Launch L;
+  std::string err;
+  if (plan_fp8(L, M, N, K, FP8_SWIGLU, err)) return fail(IXB_ERR_INVALID, err);
+  Fp8Params& p = L.p;
+  if (encode_rows(&p.tx, x, M, K, ldx, p.bn, err) || encode_rows(&p.tw[0], gate, N, K, ldg, 128, err) ||
+      encode_rows(&p.tw[1], up, N, K, ldu, 128, err))
+    return fail(IXB_ERR_CUDA, err);
+  p.xs = x_scale;
+  p.ldxs = ldxs;
+  p.ws[0] = gate_scale;
+  p.ldws[0] = ldgs;
+  p.ws[1] = up_scale;
+  p.ldws[1] = ldus;
+  if (p.m_tiles == 1) {
+    p.w[0] = gate;
+    p.ldw[0] = ldg;
+    p.w[1] = up;
+    p.ldw[1] = ldu;
+  }
+  p.q = q;
+  p.ldq = ldq;
+  p.qs = scale;
+  p.ldqs = lds;
+  return launch_fp8<FP8_SWIGLU, 2>(L, static_cast<cudaStream_t>(stream));
+}
+
+int ixb_fp8_plan_info(int M, int N, int K, int swiglu, int32_t* info, int n) {
+  if (int r = check_fp8_sizes(M, N, K)) return r;
+  if (M == 0 || !info || n < 12) return fail(IXB_ERR_INVALID, "plan info needs M >= 1 and room for 12 values");
+  Fp8Launch L;
+  std::string err;
+  if (plan_fp8(L, M, N, K, swiglu ? FP8_SWIGLU : FP8_LINEAR, err)) return fail(IXB_ERR_INVALID, err);
+  const Fp8Params& p = L.p;
+  const int32_t v[12] = {L.mt, p.bn, p.n_tiles, p.m_tiles, p.kblocks, p.split, p.kb_split, p.stages, L.grid, L.smem, p.tmem_cols, p.nacc};
+  std::copy(v, v + 12, info);
+  return IXB_OK;
 }
 
 int ixb_decode_yolo(const ixb_decode_desc* d, const int8_t* egress, int batch, uint64_t egress_image_bytes,

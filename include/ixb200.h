@@ -26,6 +26,8 @@
  *                        int8 x packed int4 -> int32 (kernels/w4a8_probe/w4a8_kernels.cc:288-305,
  *                        mm_i8i4_native; operand packing w4a8_probe.py:197-201) plus a
  *                        group-aligned pow2 SRS epilogue.
+ * ixb_fp8_* and ixb_rmsnorm_quant have no counterpart there: the 8-bit float form of the same
+ * linears, and the norm that makes their (and the int8 products') activations.
  */
 #ifndef IXB200_H
 #define IXB200_H
@@ -46,7 +48,7 @@ extern "C" {
 #define IXB_ERR_CAPACITY -6   /* more detections survive NMS than the session's capacity */
 
 #define IXB_MAX_SEGS 4
-#define IXB_API_VERSION 9
+#define IXB_API_VERSION 10
 
 /* Conv A-operand modes. */
 #define IXB_MODE_WINDOW 0   /* stride 1, same-resolution inputs: one bulk-copied pixel window per chunk */
@@ -287,6 +289,47 @@ int ixb_w4a8_gemv(const int8_t* a, const uint8_t* image, const int32_t* shift, i
  * out int32 [M][N] = sum_k a[m][k] * (w[k][n] << d), a uint8 [M][K], the weight image of
  * ixb_w4a8_prepare (equal group positions give d = 0, the plain product), K <= 32768. */
 int ixb_u8i4_gemm_i32(const uint8_t* a, const uint8_t* image, int32_t* out, int M, int N, int K, void* stream);
+
+/* fp8 linears of a decoder layer: e4m3 values with power-of-two scales for blocks of 128. A scale is
+ * one byte s standing for 2^(s - 127) (e8m0; 255 is NaN). Activations have one per 128 consecutive
+ * values of a row, scale [M][ceil(K/128)]; weights one per 128 rows x 128 columns,
+ * [ceil(N/128)][ceil(K/128)]; the last block of a row or column may be short. Values are the OCP e4m3
+ * (largest 448, no infinities). Strides (ld...) are in elements between rows. Device pointers;
+ * matrices 16-byte aligned with row strides that are multiples of 16 bytes (scales and the output of
+ * ixb_fp8_linear: any). K a multiple of 16, any M (0 returns at once). Enqueued on `stream`, with
+ * programmatic dependent launch as ixb_w4a8_gemv; capture-safe, no allocation, no workspace. */
+#define IXB_BF16 0
+#define IXB_F16 1
+#define IXB_F32 2
+/* x [M][K] of `type` -> q [M][K], scale; block_rows 1 (activations) or 128 (weights). The scale is the
+ * least power of two >= 2^-127 that brings the block's largest finite |x| to 448 or less, the rounding
+ * to nearest even; values that are not finite become NaN. */
+int ixb_fp8_quantize(const void* x, int type, int64_t ldx, int M, int K, int block_rows, uint8_t* q, int64_t ldq,
+                     uint8_t* scale, int64_t lds, void* stream);
+/* h = x + residual (rounded once, to `type`), y = (x + residual) / sqrt(mean((x + residual)^2) + eps) * weight
+ * in fp32, quantised to e4m3 with scales as above, or, with scale NULL, to int8 at a power-of-two
+ * position in [-64, 64]: q = clamp(rne(y * 2^position), -128, 127), the activations of ixb_w4a8_gemm,
+ * ixb_w4a8_gemv and ixb_i8gemm_srs. residual and h may both be NULL (y from x alone); h may be x or
+ * residual itself. weight [K] has the type of x or fp32; K at most 32768. */
+int ixb_rmsnorm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int type,
+                      int weight_type, int M, int K, float eps, int position, void* h, int64_t ldh, uint8_t* q, int64_t ldq,
+                      uint8_t* scale, int64_t lds, void* stream);
+/* out [M][N] of out_type = x . w^T: x [M][K] with its scales, w [N][K] with its blocks'. Sums in fp32 on the
+ * tensor cores (tcgen05 kind::mxf8f6f4, which multiplies the scales in), one rounding at the end. The
+ * order of a sum depends on M, N and K alone. N in [1, 2^24], K at most 2^20. */
+int ixb_fp8_linear(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* w, int64_t ldw,
+                   const uint8_t* w_scale, int64_t ldws, void* out, int out_type, int64_t ldo, int M, int N, int K,
+                   void* stream);
+/* y = silu(x . gate^T) * (x . up^T), quantised per 128 outputs of a row: q [M][N], scale [M][ceil(N/128)],
+ * the next product's x. The products stay in fp32 inside the kernel. N a multiple of 16. */
+int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* gate,
+                          int64_t ldg, const uint8_t* gate_scale, int64_t ldgs, const uint8_t* up, int64_t ldu,
+                          const uint8_t* up_scale, int64_t ldus, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int M,
+                          int N, int K, void* stream);
+/* The launch plan of a product (host only, no GPU needed): {128-row weight blocks per tile, tokens per
+ * tile, N tiles, M tiles, K blocks, CTAs per tile along K, K blocks of each, stages, grid, shared bytes,
+ * TMEM columns, accumulators}. */
+int ixb_fp8_plan_info(int M, int N, int K, int swiglu, int32_t* info, int n);
 
 /* YOLOv8 detect decode + NMS on the GPU: the detections of the reference's
  * pipelines/decode_native.c yolo_decode_int8 (:407-540), bit for bit, for `batch` images of int8
