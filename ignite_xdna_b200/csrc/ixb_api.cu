@@ -1029,11 +1029,12 @@ int encode_rows(CUtensorMap* map, const void* base, long long rows, int K, long 
 
 struct Fp8Launch {
   Fp8Params p;
-  int mt, grid, smem;
+  int mt, cg, grid, smem;
 };
 
-// Tile (MT blocks of 128 weight rows x bn tokens), split of K over a cluster, pipeline depth and
-// grid for M tokens x N outputs x K: the choice with the least estimated SM cycles.
+// Tile (MT blocks of 128 weight rows x bn tokens per CTA, a pair of CTAs sharing the tokens when cg is
+// 2), split of K over a cluster, pipeline depth and grid for M tokens x N outputs x K: the choice with
+// the least estimated SM cycles.
 int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   Fp8Params& p = L.p;
   memset(&p, 0, sizeof p);
@@ -1043,59 +1044,63 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   p.kblocks = (K + 127) / 128;
   const int sms = sm_count();
   double best = 1e300;
-  const int m16 = std::min(256, round_up(M, 16));
   const int nblk = (N + 127) / 128;
-  for (int mt : {1, 2}) {
-    if (mode == FP8_SWIGLU ? mt == 1 : (mt == 2 && nblk == 1)) continue;
-    const long long n_tiles = mode == FP8_SWIGLU ? nblk : (nblk + mt - 1) / mt;
-    for (int bn = 16; bn <= m16; bn += 16) {
-      const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
-      if (mt * bn + sf_cols > 512) break;
-      const long long tiles = n_tiles * ((M + bn - 1) / bn);
-      const int stage = mt * kGemmABlock + bn * 128;
-      for (int split : {1, 2, 4, 8}) {
-        const int kbs = (p.kblocks + split - 1) / split;
-        if (split > 1 && ((long long)(split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms ||
-                          mt * bn * 512 > std::min(kFp8MaxStages, 180 * 1024 / stage) * stage))
-          break;
-        const long long waves = (tiles * split + sms - 1) / sms;
-        const bool two = split == 1 && waves > 1 && 2 * mt * bn + sf_cols <= 512;
-        const double mma = mt * std::max(2.0 * bn, 128.0), load = stage / 45.0;
-        const double epi = 8.0 * mt * bn / (split > 1 ? 2 : 1) + (split > 1 ? 1500.0 : 0.0);
-        const double cost = waves * (kbs * std::max(mma, load) + (two ? 0.0 : epi)) + (two ? epi : 0.0);
-        if (cost < best) {
-          best = cost;
-          L.mt = mt;
-          p.bn = bn;
-          p.split = split;
-          p.kb_split = kbs;
-          p.nacc = two ? 2 : 1;
+  for (int cg : {1, 2}) {
+    if (cg == 2 && (nblk == 1 || sms < 2)) continue;
+    for (int mt : {1, 2}) {
+      if (mode == FP8_SWIGLU ? mt == 1 : mt == 2 && nblk <= cg) continue;
+      const int rows = cg * (mode == FP8_SWIGLU ? 1 : mt);  // weight blocks per tile (of each product)
+      const long long n_tiles = (nblk + rows - 1) / rows;
+      const int step = 16 * cg;
+      for (int bn = step; bn <= std::min(256, round_up(M, step)); bn += step) {
+        const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
+        if (mt * bn + sf_cols > 512) break;
+        const long long tiles = n_tiles * ((M + bn - 1) / bn);
+        const int stage = mt * kGemmABlock + bn * 128 / cg;
+        for (int split : {1, 2, 4, 8}) {
+          const int kbs = (p.kblocks + split - 1) / split;
+          if (split > 1 && (cg == 2 || (long long)(split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms ||
+                            mt * bn * 512 > std::min(kFp8MaxStages, 180 * 1024 / stage) * stage))
+            break;
+          const long long waves = cg == 2 ? (tiles + sms / 2 - 1) / (sms / 2) : (tiles * split + sms - 1) / sms;
+          const bool two = split == 1 && waves > 1 && 2 * mt * bn + sf_cols <= 512;
+          const double mma = mt * std::max(2.0 * bn, 128.0), load = stage / 45.0;
+          const double epi = 8.0 * mt * bn / (split > 1 ? 2 : 1) + (split > 1 ? 1500.0 : 0.0);
+          const double cost = waves * (kbs * std::max(mma, load) + (two ? 0.0 : epi)) + (two ? epi : 0.0);
+          if (cost < best) {
+            best = cost;
+            L.mt = mt;
+            L.cg = cg;
+            p.bn = bn;
+            p.split = split;
+            p.kb_split = kbs;
+            p.nacc = two ? 2 : 1;
+          }
         }
       }
     }
   }
-  const int mt = L.mt;
-  p.n_tiles = mode == FP8_SWIGLU ? nblk : (nblk + mt - 1) / mt;
+  const int mt = L.mt, cg = L.cg;
+  const int rows = cg * (mode == FP8_SWIGLU ? 1 : mt);
+  p.n_tiles = (nblk + rows - 1) / rows;
   p.m_tiles = (M + p.bn - 1) / p.bn;
   const long long tiles = (long long)p.n_tiles * p.m_tiles;
-  if (tiles * p.split > 0x7fffffffLL) {
+  if (tiles * p.split > 0x3fffffffLL) {
     err = "too many tiles";
     return -1;
   }
-  L.grid = (int)(p.split > 1 ? tiles * p.split : std::min<long long>(tiles, sms));
-  p.stage_bytes = mt * kGemmABlock + p.bn * 128;
+  // groups of n tiles that make the tiles in work at one time about as many weight rows as tokens
+  const double square = sqrt((double)sms / (cg * p.split) * p.bn / (128.0 * cg * mt));
+  const int groups_n = std::max(1, (int)ceil(p.n_tiles / std::max(1.0, square)));
+  p.n_group = (p.n_tiles + groups_n - 1) / groups_n;
+  L.grid = (int)(p.split > 1 ? tiles * p.split : cg * std::min<long long>(tiles, sms / cg));
+  p.stage_bytes = mt * kGemmABlock + p.bn * 128 / cg;
   const int groups = (p.bn + 127) / 128;
-  const int sf = kSfSlots * (mt + groups) * kSfAtom;
-  const int stg = p.split > 1 ? 0 : 2 * (mode == FP8_SWIGLU ? 2 : 1) * kFp8Chunk * 128 * 4;
-  // two CTAs per SM when a split grid has more CTAs than SMs
-  const int limit = L.grid > sms ? kSmemLimit / 2 - 1024 : kSmemLimit;
+  const int sf = kSfSlots * (kSfSpan / 4) * (mt + groups) * kSfAtom;
+  const int stg = p.split > 1 || mode == FP8_LINEAR ? 0 : kFp8TopBytes;
   const int red = p.split > 1 ? mt * p.bn * 512 : 0;
-  p.stages = std::min(kFp8MaxStages, (limit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
-  if (p.split > 1 || p.stages * p.stage_bytes < red || p.stages < 2) {
-    p.stages = std::min(kFp8MaxStages, (kSmemLimit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
-    p.stages = std::max(std::min(p.stages, p.kb_split), (red + p.stage_bytes - 1) / p.stage_bytes);
-  }
-  p.stages = std::max(p.stages, 1);
+  p.stages = std::min(kFp8MaxStages, (kSmemLimit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
+  if (p.split > 1) p.stages = std::max(std::min(p.stages, p.kb_split), (red + p.stage_bytes - 1) / p.stage_bytes);
   p.sf_off = p.stages * p.stage_bytes;
   p.stg_off = p.sf_off + sf;
   p.bar_off = p.stg_off + stg;
@@ -1104,17 +1109,17 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   const int need = p.nacc * p.acc_cols + 2 * 4 * (mt + groups);
   p.tmem_cols = 32;
   while (p.tmem_cols < need) p.tmem_cols *= 2;
-  p.idesc = umma_idesc_mxf8(128, p.bn);
-  if (L.smem > kSmemLimit || p.tmem_cols > 512) {
+  p.idesc = umma_idesc_mxf8(128 * cg, p.bn);
+  if (p.stages < 1 || L.smem > kSmemLimit || p.tmem_cols > 512) {
     err = "no tile fits";
     return -1;
   }
   return 0;
 }
 
-template <int MODE, int MT>
-int launch_fp8(const Fp8Launch& L, cudaStream_t st) {
-  if (int r = ensure_smem_limit(fp8_gemm_kernel<MODE, MT>, kSmemLimit)) return r;
+template <int MODE, int MT, int CG>
+int launch_fp8_cg(const Fp8Launch& L, cudaStream_t st) {
+  if (int r = ensure_smem_limit(fp8_gemm_kernel<MODE, MT, CG>, kSmemLimit)) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)L.grid);
   cfg.blockDim = dim3(kFp8Threads);
@@ -1126,16 +1131,30 @@ int launch_fp8(const Fp8Launch& L, cudaStream_t st) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (L.p.split > 1) {
+  const int cluster = CG == 2 ? 2 : L.p.split;
+  if (cluster > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = (unsigned)L.p.split;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  IXB_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<MODE, MT>, L.p));
+  IXB_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<MODE, MT, CG>, L.p));
   return 0;
+}
+
+// Whether the gatherer may copy scales as 4-byte words: aligned rows, and parts of K that start on a word.
+bool scale_words(const void* s, long long ld, const Fp8Params& p) {
+  return (reinterpret_cast<uintptr_t>(s) & 3) == 0 && ld % 4 == 0 && (p.split == 1 || p.kb_split % 4 == 0);
+}
+
+template <int MODE, int MT>
+int launch_fp8(Fp8Launch& L, cudaStream_t st) {
+  Fp8Params& p = L.p;
+  p.sf_words = scale_words(p.ws[0], p.ldws[0], p) && (MODE == FP8_LINEAR || scale_words(p.ws[1], p.ldws[1], p)) &&
+               scale_words(p.xs, p.ldxs, p);
+  return L.cg == 2 ? launch_fp8_cg<MODE, MT, 2>(L, st) : launch_fp8_cg<MODE, MT, 1>(L, st);
 }
 
 // What both products check of an operand: an e4m3 [rows][K] matrix and its scales.
@@ -2456,7 +2475,7 @@ int ixb_fp8_linear(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   std::string err;
   if (plan_fp8(L, M, N, K, FP8_LINEAR, err)) return fail(IXB_ERR_INVALID, err);
   Fp8Params& p = L.p;
-  if (encode_rows(&p.tx, x, M, K, ldx, p.bn, err) || encode_rows(&p.tw[0], w, N, K, ldw, 128, err))
+  if (encode_rows(&p.tx, x, M, K, ldx, p.bn / L.cg, err) || encode_rows(&p.tw[0], w, N, K, ldw, 128, err))
     return fail(IXB_ERR_CUDA, err);
   p.xs = x_scale;
   p.ldxs = ldxs;
@@ -2488,7 +2507,7 @@ int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale,
   std::string err;
   if (plan_fp8(L, M, N, K, FP8_SWIGLU, err)) return fail(IXB_ERR_INVALID, err);
   Fp8Params& p = L.p;
-  if (encode_rows(&p.tx, x, M, K, ldx, p.bn, err) || encode_rows(&p.tw[0], gate, N, K, ldg, 128, err) ||
+  if (encode_rows(&p.tx, x, M, K, ldx, p.bn / L.cg, err) || encode_rows(&p.tw[0], gate, N, K, ldg, 128, err) ||
       encode_rows(&p.tw[1], up, N, K, ldu, 128, err))
     return fail(IXB_ERR_CUDA, err);
   p.xs = x_scale;
@@ -2512,13 +2531,13 @@ int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale,
 
 int ixb_fp8_plan_info(int M, int N, int K, int swiglu, int32_t* info, int n) {
   if (int r = check_fp8_sizes(M, N, K)) return r;
-  if (M == 0 || !info || n < 12) return fail(IXB_ERR_INVALID, "plan info needs M >= 1 and room for 12 values");
+  if (M == 0 || !info || n < 13) return fail(IXB_ERR_INVALID, "plan info needs M >= 1 and room for 13 values");
   Fp8Launch L;
   std::string err;
   if (plan_fp8(L, M, N, K, swiglu ? FP8_SWIGLU : FP8_LINEAR, err)) return fail(IXB_ERR_INVALID, err);
   const Fp8Params& p = L.p;
-  const int32_t v[12] = {L.mt, p.bn, p.n_tiles, p.m_tiles, p.kblocks, p.split, p.kb_split, p.stages, L.grid, L.smem, p.tmem_cols, p.nacc};
-  std::copy(v, v + 12, info);
+  const int32_t v[13] = {L.cg, L.mt, p.bn, p.n_tiles, p.m_tiles, p.kblocks, p.split, p.kb_split, p.stages, L.grid, L.smem, p.tmem_cols, p.nacc};
+  std::copy(v, v + 13, info);
   return IXB_OK;
 }
 

@@ -66,6 +66,12 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
+def _scales(rows, cols, device):
+    """An empty scale matrix whose rows start on 4 bytes, which the products read a word at a time."""
+    n = _blocks(cols)
+    return torch.empty((rows, -(-n // 4) * 4), dtype=E8M0, device=device)[:, :n]
+
+
 def quantize(x, block_rows: int = 1):
     """``(q, scale)`` of a bf16, fp16 or fp32 matrix: e4m3 with a scale per 1 x 128 values
     (``block_rows=1``, activations) or per 128 x 128 (``block_rows=128``, weights). A scale is the
@@ -76,9 +82,9 @@ def quantize(x, block_rows: int = 1):
     px, ldx = _rows(x, "x")
     M, K = x.shape
     q = torch.empty((M, K), dtype=E4M3, device=x.device)
-    scale = torch.empty((M if block_rows == 1 else _blocks(M), _blocks(K)), dtype=E8M0, device=x.device)
+    scale = _scales(M if block_rows == 1 else _blocks(M), K, x.device)
     _call("ixb_fp8_quantize", x.device, px, _TYPES[x.dtype], ldx, M, K, block_rows, q.data_ptr(), K, scale.data_ptr(),
-          scale.shape[1])
+          scale.stride(0))
     return q, scale
 
 
@@ -102,10 +108,10 @@ def rmsnorm_quant(x, weight, eps: float = 1e-6, residual=None, position=None):
         pr, ldr = _rows(residual, "residual", x.dtype, x.shape)
         h = torch.empty((M, K), dtype=x.dtype, device=x.device)
     q = torch.empty((M, K), dtype=E4M3 if position is None else torch.int8, device=x.device)
-    scale = torch.empty((M, _blocks(K)), dtype=E8M0, device=x.device) if position is None else None
+    scale = _scales(M, K, x.device) if position is None else None
     _call("ixb_rmsnorm_quant", x.device, px, ldx, pr, ldr, weight.data_ptr(), _TYPES[x.dtype], _TYPES[weight.dtype], M, K,
           eps, 0 if position is None else position, None if h is None else h.data_ptr(), K, q.data_ptr(), K,
-          None if scale is None else scale.data_ptr(), _blocks(K))
+          None if scale is None else scale.data_ptr(), 0 if scale is None else scale.stride(0))
     return q, scale, h
 
 
@@ -152,6 +158,6 @@ def linear_swiglu(x, x_scale, gate, gate_scale, up, up_scale):
         raise ValueError(f"gate and up have {N} and {up.shape[0]} rows")
     _same_device(x, x_scale, gate, gate_scale, up, up_scale)
     q = torch.empty((M, N), dtype=E4M3, device=x.device)
-    scale = torch.empty((M, _blocks(N)), dtype=E8M0, device=x.device)
-    _call("ixb_fp8_linear_swiglu", x.device, *ax, *ag, *au, q.data_ptr(), N, scale.data_ptr(), _blocks(N), M, N, K)
+    scale = _scales(M, N, x.device)
+    _call("ixb_fp8_linear_swiglu", x.device, *ax, *ag, *au, q.data_ptr(), N, scale.data_ptr(), scale.stride(0), M, N, K)
     return q, scale

@@ -326,8 +326,8 @@ int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale,
                           int64_t ldg, const uint8_t* gate_scale, int64_t ldgs, const uint8_t* up, int64_t ldu,
                           const uint8_t* up_scale, int64_t ldus, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, int M,
                           int N, int K, void* stream);
-/* The launch plan of a product (host only, no GPU needed): {128-row weight blocks per tile, tokens per
- * tile, N tiles, M tiles, K blocks, CTAs per tile along K, K blocks of each, stages, grid, shared bytes,
+/* The launch plan of a product (host only, no GPU needed): {CTAs that share a tile's tokens (1 or 2),
+ * 128-row weight blocks per CTA, tokens per tile, N tiles, M tiles, K blocks, CTAs per tile along K, K blocks of each, stages, grid, shared bytes,
  * TMEM columns, accumulators}. */
 int ixb_fp8_plan_info(int M, int N, int K, int swiglu, int32_t* info, int n);
 

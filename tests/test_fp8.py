@@ -9,12 +9,12 @@ import fp8_model as F
 from ignite_xdna_b200 import _lib as L
 from ignite_xdna_b200 import fp8
 
-FIELDS = ("mt", "bn", "n_tiles", "m_tiles", "kblocks", "split", "kb_split", "stages", "grid", "smem", "tmem", "nacc")
+FIELDS = ("cg", "mt", "bn", "n_tiles", "m_tiles", "kblocks", "split", "kb_split", "stages", "grid", "smem", "tmem", "nacc")
 
 
 def plan(M, N, K, swiglu):
-    info = (C.c_int32 * 12)()
-    L.check(L.load().ixb_fp8_plan_info(M, N, K, swiglu, info, 12))
+    info = (C.c_int32 * 13)()
+    L.check(L.load().ixb_fp8_plan_info(M, N, K, swiglu, info, 13))
     return dict(zip(FIELDS, info))
 
 
@@ -28,25 +28,26 @@ def test_plans_fit_the_hardware(swiglu):
                 p = plan(M, N, K, swiglu)
                 groups = -(-p["bn"] // 128)
                 assert p["bn"] % 16 == 0 and 16 <= p["bn"] <= 256 and p["mt"] in (1, 2)
-                assert p["m_tiles"] * p["bn"] >= M and p["n_tiles"] * 128 * (1 if swiglu else p["mt"]) >= N
+                assert p["cg"] in (1, 2) and p["bn"] % (16 * p["cg"]) == 0 and (p["cg"] == 1 or p["split"] == 1)
+                assert p["m_tiles"] * p["bn"] >= M and p["n_tiles"] * 128 * p["cg"] * (1 if swiglu else p["mt"]) >= N
                 assert p["kblocks"] * 128 >= K and p["stages"] >= 1 and p["smem"] <= 227 * 1024
                 assert p["nacc"] * p["mt"] * p["bn"] + 8 * (p["mt"] + groups) <= p["tmem"] <= 512
                 assert p["tmem"] & (p["tmem"] - 1) == 0
                 # every CTA of a cluster has K-blocks of its own, and together they have all
                 assert (p["split"] - 1) * p["kb_split"] < p["kblocks"] <= p["split"] * p["kb_split"]
                 tiles = p["n_tiles"] * p["m_tiles"]
-                assert p["grid"] == tiles * p["split"] if p["split"] > 1 else 1 <= p["grid"] <= min(tiles, 148)
+                assert p["grid"] == tiles * p["split"] if p["split"] > 1 else p["cg"] <= p["grid"] <= min(tiles * p["cg"], 148)
                 if p["split"] > 1:  # the parts to add fit where the operands were
                     assert p["mt"] * p["bn"] * 512 <= p["stages"] * (p["mt"] * 16384 + p["bn"] * 128)
 
 
 def test_plan_refuses_bad_sizes():
-    info = (C.c_int32 * 12)()
+    info = (C.c_int32 * 13)()
     lib = L.load()
     for M, N, K in [(0, 16, 16), (-1, 16, 16), (16, 0, 16), (16, 16, 8), (16, 16, 24), (16, 16, 0), (1, 1 << 25, 16),
                     (1, 16, (1 << 20) + 16)]:
-        assert lib.ixb_fp8_plan_info(M, N, K, 0, info, 12) == L.IXB_ERR_INVALID, (M, N, K)
-    assert lib.ixb_fp8_plan_info(16, 16, 16, 0, info, 11) == L.IXB_ERR_INVALID
+        assert lib.ixb_fp8_plan_info(M, N, K, 0, info, 13) == L.IXB_ERR_INVALID, (M, N, K)
+    assert lib.ixb_fp8_plan_info(16, 16, 16, 0, info, 12) == L.IXB_ERR_INVALID
 
 
 P, ODD = 4096, 4104  # pointers that are never followed: every call below is refused on the host

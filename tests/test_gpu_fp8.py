@@ -166,7 +166,7 @@ def test_norm_in_place(M):
     q0, s0, h0 = fp8.rmsnorm_quant(x, w, residual=r)
     for at in (x.clone(), r.clone()):
         own_x, own_r = (at, r) if torch.equal(at, x) else (x, at)
-        q, s = torch.empty_like(q0), torch.empty_like(s0)
+        q, s = torch.empty_like(q0), torch.empty((M, 9), dtype=s0.dtype, device="cuda")
         L.check(L.load().ixb_rmsnorm_quant(own_x.data_ptr(), 1040, own_r.data_ptr(), 1040, w.data_ptr(), L.F16, L.F16, M, 1040, 1e-6,
                                            0, at.data_ptr(), 1040, q.data_ptr(), 1040, s.data_ptr(), 9, None))
         settle()
