@@ -1032,9 +1032,9 @@ struct Fp8Launch {
   int mt, cg, grid, smem;
 };
 
-// Tile (MT blocks of 128 weight rows x bn tokens per CTA, a pair of CTAs sharing the tokens when cg is
-// 2), split of K over a cluster, pipeline depth and grid for M tokens x N outputs x K: the choice with
-// the least estimated SM cycles.
+// The form (cg 1: few tokens, 2: pairs), tile (MT blocks of 128 weight rows x bn tokens per CTA), split of
+// K over a cluster, pipeline depth and grid for M tokens x N outputs x K: the choice with the least
+// estimated SM cycles.
 int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   Fp8Params& p = L.p;
   memset(&p, 0, sizeof p);
@@ -1043,41 +1043,47 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   p.K = K;
   p.kblocks = (K + 127) / 128;
   const int sms = sm_count();
-  double best = 1e300;
   const int nblk = (N + 127) / 128;
-  for (int cg : {1, 2}) {
-    if (cg == 2 && (nblk == 1 || sms < 2)) continue;
-    for (int mt : {1, 2}) {
-      if (mode == FP8_SWIGLU ? mt == 1 : mt == 2 && nblk <= cg) continue;
-      const int rows = cg * (mode == FP8_SWIGLU ? 1 : mt);  // weight blocks per tile (of each product)
-      const long long n_tiles = (nblk + rows - 1) / rows;
-      const int step = 16 * cg;
-      for (int bn = step; bn <= std::min(256, round_up(M, step)); bn += step) {
-        const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
-        if (mt * bn + sf_cols > 512) break;
-        const long long tiles = n_tiles * ((M + bn - 1) / bn);
-        const int stage = mt * kGemmABlock + bn * 128 / cg;
-        for (int split : {1, 2, 4, 8}) {
-          const int kbs = (p.kblocks + split - 1) / split;
-          if (split > 1 && (cg == 2 || (long long)(split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms ||
-                            mt * bn * 512 > std::min(kFp8MaxStages, 180 * 1024 / stage) * stage))
-            break;
-          const long long waves = cg == 2 ? (tiles + sms / 2 - 1) / (sms / 2) : (tiles * split + sms - 1) / sms;
-          const bool two = split == 1 && waves > 1 && 2 * mt * bn + sf_cols <= 512;
-          const double mma = mt * std::max(2.0 * bn, 128.0), load = stage / 45.0;
-          const double epi = 8.0 * mt * bn / (split > 1 ? 2 : 1) + (split > 1 ? 1500.0 : 0.0);
-          const double cost = waves * (kbs * std::max(mma, load) + (two ? 0.0 : epi)) + (two ? epi : 0.0);
-          if (cost < best) {
-            best = cost;
-            L.mt = mt;
-            L.cg = cg;
-            p.bn = bn;
-            p.split = split;
-            p.kb_split = kbs;
-            p.nacc = two ? 2 : 1;
-          }
-        }
+  double best = 1e300;
+  auto take = [&](double cost, int cg, int mt, int bn, int split, int kbs, int nacc) {
+    if (cost >= best) return;
+    best = cost;
+    L.cg = cg;
+    L.mt = mt;
+    p.bn = bn;
+    p.split = split;
+    p.kb_split = kbs;
+    p.nacc = nacc;
+  };
+  // Few tokens: a CTA per tile and part of K. An SM takes the CTAs that fall to it one K-block in ~150
+  // cycles or at the rate its operands arrive; adding the parts of a split costs a cluster's barriers.
+  {
+    const int mt = mode == FP8_SWIGLU ? 2 : 1;
+    for (int bn = 16; bn <= std::min(kFp8FewTokens, round_up(M, 16)); bn += 16) {
+      const long long tiles = (long long)nblk * ((M + bn - 1) / bn);
+      const int stage = mt * kGemmABlock + bn * 128;
+      for (int split = 1; split <= kFp8MaxSplit; ++split) {
+        const int kbs = (p.kblocks + split - 1) / split;
+        if (split > 1 && ((split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms)) break;
+        const long long per_sm = (tiles * split + sms - 1) / sms;
+        const double kb = std::max(std::max(mt * std::max(2.0 * bn, 128.0), stage / 40.0), 150.0);
+        take(per_sm * kbs * kb + 2500.0 + 4.0 * mt * bn + (split > 1 ? 700.0 : 0.0), 1, mt, bn, split, kbs, 1);
       }
+    }
+  }
+  // Many tokens: persistent pairs.
+  for (int mt : {1, 2}) {
+    if ((mode == FP8_SWIGLU && mt == 1) || sms < 2) continue;
+    const int rows = 2 * (mode == FP8_SWIGLU ? 1 : mt);  // weight blocks per tile (of each product)
+    for (int bn = 32; bn <= std::min(256, round_up(M, 32)); bn += 32) {
+      const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
+      if (mt * bn + sf_cols > 512) break;
+      const long long tiles = (long long)((nblk + rows - 1) / rows) * ((M + bn - 1) / bn);
+      const long long waves = (tiles + sms / 2 - 1) / (sms / 2);
+      const bool two = waves > 1 && 2 * mt * bn + sf_cols <= 512;
+      const double kb = std::max(mt * 2.0 * bn + 60.0, 520.0);
+      const double epi = 14.0 * mt * bn;
+      take(waves * (p.kblocks * kb + (two ? 0.0 : epi)) + (two ? epi : 0.0) + 4000.0, 2, mt, bn, 1, p.kblocks, two ? 2 : 1);
     }
   }
   const int mt = L.mt, cg = L.cg;
@@ -1093,24 +1099,26 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   const double square = sqrt((double)sms / (cg * p.split) * p.bn / (128.0 * cg * mt));
   const int groups_n = std::max(1, (int)ceil(p.n_tiles / std::max(1.0, square)));
   p.n_group = (p.n_tiles + groups_n - 1) / groups_n;
-  L.grid = (int)(p.split > 1 ? tiles * p.split : cg * std::min<long long>(tiles, sms / cg));
+  L.grid = (int)(cg == 1 ? tiles * p.split : 2 * std::min<long long>(tiles, sms / 2));
   p.stage_bytes = mt * kGemmABlock + p.bn * 128 / cg;
   const int groups = (p.bn + 127) / 128;
   const int sf = kSfSlots * (kSfSpan / 4) * (mt + groups) * kSfAtom;
-  const int stg = p.split > 1 || mode == FP8_LINEAR ? 0 : kFp8TopBytes;
-  const int red = p.split > 1 ? mt * p.bn * 512 : 0;
-  p.stages = std::min(kFp8MaxStages, (kSmemLimit - 1024 - sf - stg - kFp8BarBytes) / p.stage_bytes);
-  if (p.split > 1) p.stages = std::max(std::min(p.stages, p.kb_split), (red + p.stage_bytes - 1) / p.stage_bytes);
+  const int stg = cg == 2 && mode == FP8_SWIGLU ? kFp8TopBytes : 0;
+  const int fixed = 1024 + sf + stg + kFp8BarBytes;
+  // the few-token form leaves room for a second CTA (1 KB of each SM's 228 is the system's, per CTA)
+  const int limit = cg == 1 ? kSmemLimit / 2 - 1024 : kSmemLimit;
+  const int red = cg == 1 ? (mt * p.bn * 512 + p.stage_bytes - 1) / p.stage_bytes : 1;
+  p.stages = std::max(std::min(std::min(kFp8MaxStages, (limit - fixed) / p.stage_bytes), p.kb_split), red);
   p.sf_off = p.stages * p.stage_bytes;
   p.stg_off = p.sf_off + sf;
   p.bar_off = p.stg_off + stg;
-  L.smem = 1024 + p.bar_off + kFp8BarBytes;
+  L.smem = fixed + p.sf_off;
   p.acc_cols = mt * p.bn;
   const int need = p.nacc * p.acc_cols + 2 * 4 * (mt + groups);
   p.tmem_cols = 32;
   while (p.tmem_cols < need) p.tmem_cols *= 2;
   p.idesc = umma_idesc_mxf8(128 * cg, p.bn);
-  if (p.stages < 1 || L.smem > kSmemLimit || p.tmem_cols > 512) {
+  if (L.smem > kSmemLimit || p.tmem_cols > 512 || p.stages > kFp8MaxStages) {
     err = "no tile fits";
     return -1;
   }
@@ -1149,12 +1157,13 @@ bool scale_words(const void* s, long long ld, const Fp8Params& p) {
   return (reinterpret_cast<uintptr_t>(s) & 3) == 0 && ld % 4 == 0 && (p.split == 1 || p.kb_split % 4 == 0);
 }
 
-template <int MODE, int MT>
-int launch_fp8(Fp8Launch& L, cudaStream_t st) {
+int launch_fp8(Fp8Launch& L, int mode, cudaStream_t st) {
   Fp8Params& p = L.p;
-  p.sf_words = scale_words(p.ws[0], p.ldws[0], p) && (MODE == FP8_LINEAR || scale_words(p.ws[1], p.ldws[1], p)) &&
+  p.sf_words = scale_words(p.ws[0], p.ldws[0], p) && (mode == FP8_LINEAR || scale_words(p.ws[1], p.ldws[1], p)) &&
                scale_words(p.xs, p.ldxs, p);
-  return L.cg == 2 ? launch_fp8_cg<MODE, MT, 2>(L, st) : launch_fp8_cg<MODE, MT, 1>(L, st);
+  if (mode == FP8_SWIGLU) return L.cg == 2 ? launch_fp8_cg<FP8_SWIGLU, 2, 2>(L, st) : launch_fp8_cg<FP8_SWIGLU, 2, 1>(L, st);
+  if (L.cg == 1) return launch_fp8_cg<FP8_LINEAR, 1, 1>(L, st);
+  return L.mt == 1 ? launch_fp8_cg<FP8_LINEAR, 1, 2>(L, st) : launch_fp8_cg<FP8_LINEAR, 2, 2>(L, st);
 }
 
 // What both products check of an operand: an e4m3 [rows][K] matrix and its scales.
@@ -1167,8 +1176,8 @@ int check_fp8_operand(const void* v, int64_t ld, const void* s, int64_t lds, int
 }
 
 int check_fp8_sizes(int M, int N, int K) {
-  if (M < 0 || N < 1 || K < 16 || K % 16 || K > (1 << 20) || N > (1 << 24))
-    return fail(IXB_ERR_INVALID, "fp8 product needs M >= 0, N in [1, 2^24], K a multiple of 16 in [16, 2^20]");
+  if (M < 0 || N < 1 || K < 16 || K % 16 || K > 65536 || N > (1 << 24))
+    return fail(IXB_ERR_INVALID, "fp8 product needs M >= 0, N in [1, 2^24], K a multiple of 16 in [16, 65536]");
   return 0;
 }
 
@@ -2481,15 +2490,14 @@ int ixb_fp8_linear(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   p.ldxs = ldxs;
   p.ws[0] = w_scale;
   p.ldws[0] = ldws;
-  if (p.m_tiles == 1) {
+  if (L.cg == 1 && p.m_tiles == 1) {
     p.w[0] = w;
     p.ldw[0] = ldw;
   }
   p.out = out;
   p.out_type = out_type;
   p.ldo = ldo;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return L.mt == 1 ? launch_fp8<FP8_LINEAR, 1>(L, st) : launch_fp8<FP8_LINEAR, 2>(L, st);
+  return launch_fp8(L, FP8_LINEAR, static_cast<cudaStream_t>(stream));
 }
 
 int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* gate,
@@ -2516,7 +2524,7 @@ int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale,
   p.ldws[0] = ldgs;
   p.ws[1] = up_scale;
   p.ldws[1] = ldus;
-  if (p.m_tiles == 1) {
+  if (L.cg == 1 && p.m_tiles == 1) {
     p.w[0] = gate;
     p.ldw[0] = ldg;
     p.w[1] = up;
@@ -2526,7 +2534,7 @@ int ixb_fp8_linear_swiglu(const uint8_t* x, int64_t ldx, const uint8_t* x_scale,
   p.ldq = ldq;
   p.qs = scale;
   p.ldqs = lds;
-  return launch_fp8<FP8_SWIGLU, 2>(L, static_cast<cudaStream_t>(stream));
+  return launch_fp8(L, FP8_SWIGLU, static_cast<cudaStream_t>(stream));
 }
 
 int ixb_fp8_plan_info(int M, int N, int K, int swiglu, int32_t* info, int n) {

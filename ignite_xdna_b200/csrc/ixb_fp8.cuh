@@ -300,11 +300,16 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
 // warp gathers them from global memory into a 512-byte shared-memory image per 128 rows, and
 // tcgen05.cp (32x128b, warpx4) brings that into TMEM, in order before the MMAs that read it.
 //
-// Few tokens leave few tiles: a cluster of `split` CTAs then shares a tile along K and adds its
-// 32-bit parts in rank order over distributed shared memory.
+// Two forms. Few tokens (CG 1): tiles of at most 128 tokens, one per CTA or cluster; a cluster of up to
+// four CTAs shares a tile along K and adds its 32-bit parts in rank order over distributed shared
+// memory; shared memory and registers leave room for two CTAs per SM, so the next kernel's start,
+// and its prefetch of its weights into L2, overlap this one's end. Many tokens (CG 2): persistent
+// pairs of CTAs.
 constexpr int kFp8Epi = 8;                               // epilogue warps, two groups of four
 constexpr int kFp8Threads = 32 * (kFp8Epi + 3);          // + TMA producer, MMA issuer, scale gatherer
 constexpr int kFp8MaxStages = 12;
+constexpr int kFp8MaxSplit = 4;                          // CTAs that share a tile along K (eight took twice as long to start)
+constexpr int kFp8FewTokens = 128;                       // tokens per tile of the split form
 constexpr int kSfSlots = 2;                              // scale images in shared memory
 constexpr int kSfSpan = 16;                              // K-blocks per image: four 32-bit words per row
 constexpr int kSfAtom = 512;                             // bytes of four K-blocks' words of 128 rows
@@ -588,7 +593,7 @@ __device__ __forceinline__ int weight_block(int nt, int pair, int b) {  // 128-r
   return MODE == FP8_SWIGLU ? nt * CG + pair : (nt * CG + pair) * MT + b;
 }
 template <int MODE, int MT, int CG>
-__global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
+__global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
   constexpr int PW = kFp8Epi, MW = kFp8Epi + 1, SW = kFp8Epi + 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -604,13 +609,14 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
   uint64_t* done = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
 
-  const int rank = CG == 1 && p.split > 1 ? (int)cluster_rank() : 0;    // part of K
-  const int pair = CG == 2 ? (int)cluster_rank() : 0;                   // part of the tile
+  const int rank = CG == 1 ? (int)cluster_rank() : 0;  // part of K
+  const int pair = CG == 2 ? (int)cluster_rank() : 0;  // part of the tile
   const int tiles = p.n_tiles * p.m_tiles;
   const int share = CG == 2 ? 2 : p.split;
   const int tile0 = blockIdx.x / share, tstep = gridDim.x / share;
   const int kb0 = rank * p.kb_split, kb1 = min(p.kblocks, kb0 + p.kb_split);  // host: kb0 < kblocks for every rank
-  const int sfb_groups = (p.bn + 127) / 128;
+  constexpr int kXRows = CG == 1 ? 4 : 8;  // x rows per lane of a scale image: bn is at most 128, or 256
+  const int sfb_groups = CG == 1 ? 1 : (p.bn + 127) / 128;
   const int sf_quad = (MT + sfb_groups) * kSfAtom;  // four K-blocks' images
 
   grid_dep_launch();
@@ -651,6 +657,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
   if (CG == 2) cluster_sync();  // both CTAs' barriers exist before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  bool part_ok = true;
   grid_dep_wait();  // x, the scales, and whatever still reads the outputs, from here on
 
   if (warp == PW) {
@@ -702,8 +709,8 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
     for (int t = tile0; ok && t < tiles; t += tstep) {
       int mt, nt;
       tile_at(p, t, mt, nt);
-      const uint8_t* row[MT + 8];  // this lane's rows: the weight blocks', then x's
-      bool in[MT + 8];
+      const uint8_t* row[MT + kXRows];  // this lane's rows: the weight blocks', then x's
+      bool in[MT + kXRows];
 #pragma unroll
       for (int b = 0; b < MT; ++b) {
         const int src = MODE == FP8_SWIGLU ? b : 0;
@@ -712,7 +719,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
         row[b] = p.ws[src] + (in[b] ? r : 0) * p.ldws[src];
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kXRows; ++j) {
         const long long m = (long long)mt * p.bn + j * 32 + lane;
         in[MT + j] = j * 32 + lane < p.bn && m < p.M;
         row[MT + j] = p.xs + (in[MT + j] ? m : 0) * p.ldxs;
@@ -728,7 +735,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
           const int left = min(4, p.kblocks - kq);
           if (p.sf_words) {
 #pragma unroll
-            for (int i = 0; i < MT + 8; ++i) {
+            for (int i = 0; i < MT + kXRows; ++i) {
               if (i >= MT + 4 && sfb_groups == 1) continue;
 #pragma unroll
               for (int j = 0; j < (i < MT ? 4 : 1); ++j)
@@ -736,14 +743,14 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
                            in[i] ? left : 0);
             }
           } else {
-            uint32_t w[MT + 8];
+            uint32_t w[MT + kXRows];
 #pragma unroll
-            for (int i = 0; i < MT + 8; ++i) w[i] = scale_bytes(row[i] + kq, left);
+            for (int i = 0; i < MT + kXRows; ++i) w[i] = scale_bytes(row[i] + kq, left);
 #pragma unroll
             for (int i = 0; i < MT; ++i)
               *reinterpret_cast<uint4*>(im + i * kSfAtom) = in[i] ? make_uint4(w[i], w[i], w[i], w[i]) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < kXRows / 4; ++g) {
               const int i = MT + 4 * g;
               if (g < sfb_groups)
                 *reinterpret_cast<uint4*>(im + (MT + g) * kSfAtom) =
@@ -848,7 +855,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
         mbar_poll(done, 0);
       }
     }
-  } else if (p.split == 1) {
+  } else if constexpr (CG == 2) {
     // ------------------------------------------------------------ epilogue
     // A warp reads 32 columns of its TMEM lane quarter at a time (a lane holds one output n of 32
     // tokens) and stores each token's 32 outputs as one run; the two groups of four warps take
@@ -909,10 +916,11 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
       }
     }
   } else {
-    // ------------------------------------------------------------ this rank's part of a split tile
+    // ------------------------------------------------------------ this rank's part of a tile
     const int q = warp & 3, g = warp >> 2;
     float* red = reinterpret_cast<float*>(smem);  // [MT * bn][128] over the stages, which every MMA has read
-    if (mbar_poll(&acc_full[0], 0)) {
+    part_ok = mbar_poll(&acc_full[0], 0);
+    if (part_ok) {
       tc_fence_after();
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
       for (int c = g; c < MT * p.bn / 16; c += kFp8Epi / 4) {
@@ -926,9 +934,11 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
     tc_fence_before();
   }
   __syncwarp();
-  if (CG == 1 && p.split > 1) {
+  if constexpr (CG == 1) {
+    // The parts are added in rank order; each rank finishes every split-th run of eight tokens, a warp
+    // a token (128 outputs, four per lane).
     cluster_sync();
-    if (warp < kFp8Epi && !wait_timed_out()) {
+    if (warp < kFp8Epi && part_ok) {
       int mt, nt;
       tile_at(p, tile0, mt, nt);
       for (int c = rank * kFp8Epi + warp; c < p.bn; c += p.split * kFp8Epi) {
@@ -937,27 +947,31 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const __grid_c
         float4 v[MT];
 #pragma unroll
         for (int b = 0; b < MT; ++b) {
-          v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int r = 0; r < p.split; ++r) {
-            const float4 a = ld_cluster_f4(cluster_addr(smem + ((b * p.bn + c) * 128 + lane * 4) * 4, r));
-            v[b].x += a.x;
-            v[b].y += a.y;
-            v[b].z += a.z;
-            v[b].w += a.w;
-          }
-        }
-        if constexpr (MODE == FP8_SWIGLU) finish_swiglu(p, m, nt * 128 + lane * 4, v[0], v[MT - 1]);
-        else
+          float4 part[kFp8MaxSplit];
 #pragma unroll
-          for (int b = 0; b < MT; ++b) finish_linear(p, m, (nt * MT + b) * 128 + lane * 4, v[b]);
+          for (int r = 0; r < kFp8MaxSplit; ++r)
+            if (r < p.split) part[r] = ld_cluster_f4(cluster_addr(smem + ((b * p.bn + c) * 128 + lane * 4) * 4, r));
+          v[b] = part[0];
+#pragma unroll
+          for (int r = 1; r < kFp8MaxSplit; ++r)
+            if (r < p.split) {
+              v[b].x += part[r].x;
+              v[b].y += part[r].y;
+              v[b].z += part[r].z;
+              v[b].w += part[r].w;
+            }
+        }
+        if constexpr (MODE == FP8_SWIGLU) finish_swiglu(p, m, nt * 128 + lane * 4, v[0], v[1]);
+        else finish_linear(p, m, nt * 128 + lane * 4, v[0]);
       }
     }
     __syncwarp();
-    cluster_sync();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2) cluster_sync();  // neither CTA leaves while the pair's MMAs and signals reach it
+  // no CTA leaves while another reads its shared memory (parts of a tile), or while the pair's MMAs and
+  // signals reach it
+  cluster_sync();
   tc_fence_after();
   if (warp == MW) tmem_dealloc_cg<CG>(tmem, p.tmem_cols);
 }
