@@ -123,6 +123,16 @@ def test_python_refuses_what_is_not_a_cuda_matrix():
         fp8.linear(q, s, w, ws)
     with pytest.raises(ValueError, match="CUDA"):
         fp8.linear_swiglu(q, s, w, ws, w, ws)
+    with pytest.raises(TypeError, match="tensor"):
+        fp8.linear(None, s, w, ws)
+    with pytest.raises(TypeError, match="tensor"):
+        fp8.quantize([1.0])
+    with pytest.raises(TypeError):
+        fp8.quantize(x, block_rows="many")
+    with pytest.raises(ValueError, match="grad"):
+        fp8.quantize(x.clone().requires_grad_())
+    with pytest.raises(ValueError, match="strided"):
+        fp8.quantize(x.to_sparse())
 
 
 def test_the_model_rounds_as_torch_does():
