@@ -29,9 +29,6 @@ enum : int { FT_BF16 = 0, FT_F16 = 1, FT_F32 = 2 };  // IXB_BF16, IXB_F16, IXB_F
 constexpr int kQBlock = 128;                         // values that share a scale
 
 // ---------------------------------------------------------------- conversions
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(float v) { return v; }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -41,26 +38,104 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-// Eight consecutive values, 16-byte aligned.
+// Eight consecutive values as they lie in memory, 16-byte aligned, two (fp32: one) per word.
 template <typename T>
-struct alignas(16) Vec8 {
-  T v[8];
+struct Vec8 {
+  uint4 w[sizeof(T) / 2];
 };
 template <typename T>
 __device__ __forceinline__ Vec8<T> load8(const T* p) {
   Vec8<T> r;
-  const uint4* s = reinterpret_cast<const uint4*>(p);
-  uint4* d = reinterpret_cast<uint4*>(&r);
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(r) / 16); ++i) d[i] = s[i];
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const Vec8<T>& r) {
-  const uint4* s = reinterpret_cast<const uint4*>(&r);
-  uint4* d = reinterpret_cast<uint4*>(p);
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(r) / 16); ++i) d[i] = s[i];
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+}
+__device__ __forceinline__ void unpack8(const Vec8<__nv_bfloat16>& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of the fp32
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const Vec8<__half>& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ void unpack8(const Vec8<float>& v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[4 * i] = __uint_as_float(v.w[i].x);
+    f[4 * i + 1] = __uint_as_float(v.w[i].y);
+    f[4 * i + 2] = __uint_as_float(v.w[i].z);
+    f[4 * i + 3] = __uint_as_float(v.w[i].w);
+  }
+}
+__device__ __forceinline__ void pack8(const float (&f)[8], Vec8<__nv_bfloat16>& v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<__nv_bfloat162*>(&w[i]) = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  v.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void pack8(const float (&f)[8], Vec8<__half>& v) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<__half2*>(&w[i]) = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+  v.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void pack8(const float (&f)[8], Vec8<float>& v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    v.w[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                        __float_as_uint(f[4 * i + 3]));
+}
+
+// Two fp32 operations in one instruction (sm_100a), over eight values.
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split_pair(unsigned long long v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a[i], a[i + 1])), "l"(pair_of(b[i], b[i + 1])));
+    split_pair(r, a[i], a[i + 1]);
+  }
+}
+__device__ __forceinline__ void mul8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a[i], a[i + 1])), "l"(pair_of(b[i], b[i + 1])));
+    split_pair(r, a[i], a[i + 1]);
+  }
+}
+__device__ __forceinline__ void mul8(float (&a)[8], float b) {
+  const float s[8] = {b, b, b, b, b, b, b, b};
+  mul8(a, s);
+}
+__device__ __forceinline__ unsigned long long squares8(const float (&a)[8], unsigned long long sum) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const unsigned long long v = pair_of(a[i], a[i + 1]);
+    asm("fma.rn.f32x2 %0, %1, %1, %0;" : "+l"(sum) : "l"(v));
+  }
+  return sum;
 }
 
 // |v| of a finite value, 0 of another one: what sets a block's scale.
@@ -76,11 +151,9 @@ __device__ __forceinline__ uint32_t scale_byte(float top) {
 }
 // 2^(127 - s): exact for every byte scale_byte gives (0 .. 247).
 __device__ __forceinline__ float scale_inverse(uint32_t s) { return __uint_as_float((254u - s) << 23); }
-// Two values as e4m3 (lo in the low byte); what is not finite becomes NaN.
+// Two values as e4m3 (lo in the low byte): nearest even, past 448 to 448, NaN to NaN. Infinities have to
+// be NaN already (no_infinity).
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  const float nan = __uint_as_float(0x7FFFFFFFu);
-  lo = fabsf(lo) <= FLT_MAX ? lo : nan;
-  hi = fabsf(hi) <= FLT_MAX ? hi : nan;
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
@@ -88,6 +161,7 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
 }
+__device__ __forceinline__ float no_infinity(float v) { return fabsf(v) <= FLT_MAX ? v : __uint_as_float(0x7FFFFFFFu); }
 // int8 at a position: round to nearest even, saturating; NaN gives 0.
 __device__ __forceinline__ uint32_t s8x4(float a, float b, float c, float d) {
   const float v[4] = {a, b, c, d};
@@ -106,91 +180,134 @@ __device__ __forceinline__ float half_warp_max(float v) {
   return v;
 }
 
+// The largest finite |v| of the block of 128 values that a half-warp holds, eight per lane. fmaxf passes over
+// NaN; an infinity, rare, sends the warp through the finite values once more and turns it into NaN.
+__device__ __forceinline__ float block_top(float (&f)[8]) {
+  float top = fabsf(f[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+  top = half_warp_max(top);
+  if (__any_sync(0xffffffffu, !(top <= FLT_MAX))) {
+    top = finite_abs(f[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, finite_abs(f[j]));
+    top = half_warp_max(top);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = no_infinity(f[j]);
+  }
+  return top;
+}
+__device__ __forceinline__ uint2 round8(float (&f)[8], float m) {
+  mul8(f, m);
+  return make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
+}
+
 // ---------------------------------------------------------------- quantise
 // Rows in blocks of 1 x 128: 16 lanes per block, eight values per lane. Bound by HBM.
 constexpr int kQThreads = 256;
 constexpr int kQUnroll = 4;  // blocks per half-warp, so four 16-byte loads per lane are in flight
 template <typename T>
 __global__ void __launch_bounds__(kQThreads)
-    quantize_rows_kernel(const T* __restrict__ x, long long ldx, int K, int kb, long long blocks, uint8_t* __restrict__ q,
+    quantize_rows_kernel(const T* __restrict__ x, long long ldx, int K, FastDiv kb, uint32_t blocks, uint8_t* __restrict__ q,
                          long long ldq, uint8_t* __restrict__ scale, long long lds) {
   grid_dep_launch();
   grid_dep_wait();
-  const int lane = threadIdx.x & 31, l16 = lane & 15;
-  const long long hw = ((long long)blockIdx.x * kQThreads + threadIdx.x) >> 4;  // half-warp
-  const long long hws = (long long)gridDim.x * (kQThreads / 16);
-  for (long long b0 = hw; (b0 & ~1LL) < blocks; b0 += hws * kQUnroll) {  // a warp's two halves leave together
+  const int l16 = threadIdx.x & 15;
+  const uint32_t hws = gridDim.x * (kQThreads / 16);  // half-warps; even, so a warp's two halves leave together
+  for (uint32_t b0 = (blockIdx.x * kQThreads + threadIdx.x) >> 4; (b0 & ~1u) < blocks; b0 += hws * kQUnroll) {
     Vec8<T> v[kQUnroll];
-    long long row[kQUnroll];
+    uint32_t row[kQUnroll];
     int col[kQUnroll];
     bool ok[kQUnroll];
 #pragma unroll
     for (int i = 0; i < kQUnroll; ++i) {
-      const long long b = b0 + i * hws;
-      row[i] = b / kb;
-      col[i] = (int)(b - row[i] * kb) * kQBlock + l16 * 8;
+      const uint32_t b = b0 + i * hws;  // below 2^31 + 4 * 2^22: no wrap
+      row[i] = fdiv(b, kb);
+      col[i] = (int)(b - row[i] * kb.d) * kQBlock + l16 * 8;
       ok[i] = b < blocks && col[i] < K;
-      if (ok[i]) v[i] = load8(x + row[i] * ldx + col[i]);
+      v[i] = ok[i] ? load8(x + row[i] * ldx + col[i]) : Vec8<T>{};
     }
 #pragma unroll
     for (int i = 0; i < kQUnroll; ++i) {
-      float f[8], top = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f[j] = ok[i] ? to_f32(v[i].v[j]) : 0.f;
-        top = fmaxf(top, finite_abs(f[j]));
-      }
-      const uint32_t s = scale_byte(half_warp_max(top));
-      const float m = scale_inverse(s);
+      float f[8];
+      unpack8(v[i], f);
+      const uint32_t s = scale_byte(block_top(f));
       if (ok[i]) {
-        *reinterpret_cast<uint2*>(q + row[i] * ldq + col[i]) =
-            make_uint2(e4m3x4(f[0] * m, f[1] * m, f[2] * m, f[3] * m), e4m3x4(f[4] * m, f[5] * m, f[6] * m, f[7] * m));
+        *reinterpret_cast<uint2*>(q + row[i] * ldq + col[i]) = round8(f, scale_inverse(s));
         if (l16 == 0) scale[row[i] * lds + col[i] / kQBlock] = (uint8_t)s;
       }
     }
   }
 }
 
-// A weight's 128 x 128 blocks: a CTA per block, eight 16-byte vectors per thread held in registers
-// between the maximum and the rounding, so the weight is read once.
+// A weight's 128 x 128 blocks: a CTA per block, V vectors of eight per thread held in registers, as they lie
+// in memory, between the maximum and the rounding, so the weight is read once. Bound by HBM: four
+// CTAs' loads are in flight on an SM. (Kept unpacked, the values spill or leave room for two CTAs:
+// 38 and 31 us for 11008 x 4096 bf16 instead of 22.6, 5.97 TB/s.)
+constexpr int kTileThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2)
     quantize_tiles_kernel(const T* __restrict__ x, long long ldx, int M, int K, uint8_t* __restrict__ q, long long ldq,
                           uint8_t* __restrict__ scale, long long lds) {
+  constexpr int V = 128 * 128 / 8 / kTileThreads, kStep = kTileThreads / 16;  // rows between a thread's vectors
   grid_dep_launch();
   grid_dep_wait();
-  __shared__ float tops[8];
+  __shared__ float tops[2][kTileThreads / 32];
   const int tid = threadIdx.x;
   const int col = blockIdx.x * kQBlock + (tid & 15) * 8;
   const long long row0 = (long long)blockIdx.y * kQBlock + (tid >> 4);
-  Vec8<T> v[8];
+  auto in = [&](int i) { return col < K && row0 + kStep * i < M; };
+  auto block_top = [&](float top, float* part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((tid & 31) == 0) part[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTileThreads / 32; ++i) top = fmaxf(top, part[i]);
+    return top;
+  };
+  Vec8<T> v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = in(i) ? load8(x + (row0 + kStep * i) * ldx + col) : Vec8<T>{};
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col < K && row0 + 16 * i < M) v[i] = load8(x + (row0 + 16 * i) * ldx + col);
+  for (int i = 0; i < V; ++i) {
+    float f[8];
+    unpack8(v[i], f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col < K && row0 + 16 * i < M) {
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+  }
+  top = block_top(top, tops[0]);
+  const bool infinite = !(top <= FLT_MAX);  // the same in every thread
+  if (infinite) {  // rare: the finite values alone, read again
+    top = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < V; ++i)
+      if (in(i)) {
+        float f[8];
+        unpack8(load8(x + (row0 + kStep * i) * ldx + col), f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(to_f32(v[i].v[j])));
-    }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((tid & 31) == 0) tops[tid >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, tops[i]);
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(f[j]));
+      }
+    top = block_top(top, tops[1]);
+  }
   const uint32_t s = scale_byte(top);
   const float m = scale_inverse(s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col < K && row0 + 16 * i < M) {
-      float f[8];
+  for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = to_f32(v[i].v[j]) * m;
-      *reinterpret_cast<uint2*>(q + (row0 + 16 * i) * ldq + col) =
-          make_uint2(e4m3x4(f[0], f[1], f[2], f[3]), e4m3x4(f[4], f[5], f[6], f[7]));
+    for (int j = 0; j < (int)(sizeof(T) / 2); ++j)  // opaque, so that nothing unpacked is kept
+      asm volatile("" : "+r"(v[i].w[j].x), "+r"(v[i].w[j].y), "+r"(v[i].w[j].z), "+r"(v[i].w[j].w));
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float f[8];
+    unpack8(v[i], f);
+    if (infinite) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = no_infinity(f[j]);
     }
+    if (in(i)) *reinterpret_cast<uint2*>(q + (row0 + kStep * i) * ldq + col) = round8(f, m);
+  }
   if (tid == 0) scale[(long long)blockIdx.y * lds + blockIdx.x] = (uint8_t)s;
 }
 
@@ -207,81 +324,122 @@ struct NormParams {
   float eps, unit;       // unit: 2^position
 };
 
-// A CTA per row (the grid strides over the rows): V vectors of eight values per thread stay in
-// registers between the sum of squares and the output, so the row is read once. Bound by HBM for
-// many rows, by the latency of one load, two barriers and one store for few.
+// A CTA per row, the grid striding over the rows: V vectors of eight values per thread stay in registers
+// between the sum of squares and the output, so the row is read once. With many rows HBM bounds it,
+// and the next row's loads (without a residual the next two rows') are issued before this row's barrier, so
+// that they are in flight while it is reduced and rounded, and the weight stays in registers (V up to
+// 2 and 16-bit values: more would spill). With few rows: one load, one barrier and one store.
 template <typename T, typename W, int V>
 __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const __grid_constant__ NormParams p) {
+  constexpr bool kAhead = V <= 2 && sizeof(T) == 2;
   grid_dep_launch();
   grid_dep_wait();
   __shared__ float part[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int wide = 1;  // warps, rounded up to a power of two; the parts past them stay 0
+  while (wide < warps) wide *= 2;
+  if (tid < 32) part[0][tid] = part[1][tid] = 0.f;
+  __syncthreads();
+  const float inv_k = 1.f / (float)p.K;
   const T* xs = static_cast<const T*>(p.x);
   const T* rs = static_cast<const T*>(p.residual);
   const W* ws = static_cast<const W*>(p.weight);
   T* hs = static_cast<T*>(p.h);
-  int buf = 0;
-  for (long long row = blockIdx.x; row < p.M; row += gridDim.x, buf ^= 1) {
-    float f[V][8];
-    float sum = 0.f;
-    Vec8<T> a[V], r[V];
+  // a: the row's x; b: its residual, or, without one, the x of the CTA's next row
+  Vec8<T> a[V], b[V];
+  auto load = [&](Vec8<T>(&v)[V], const T* base, long long ld, long long row) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int col = (i * blockDim.x + tid) * 8;
-      if (col < p.K) {
-        a[i] = load8(xs + row * p.ldx + col);
-        if (rs) r[i] = load8(rs + row * p.ldr + col);
+      v[i] = col < p.K && row < p.M ? load8(base + row * ld + col) : Vec8<T>{};
+    }
+  };
+  const long long step = gridDim.x;
+  if (kAhead) {
+    load(a, xs, p.ldx, blockIdx.x);
+    load(b, rs ? rs : xs, rs ? p.ldr : p.ldx, rs ? blockIdx.x : blockIdx.x + step);
+  }
+  Vec8<W> wv[V];
+  auto load_weight = [&] {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int col = (i * blockDim.x + tid) * 8;
+      wv[i] = col < p.K ? load8(ws + col) : Vec8<W>{};
+    }
+  };
+  if (kAhead) load_weight();
+  int buf = 0;
+  for (long long row = blockIdx.x; row < p.M; row += step, buf ^= 1) {
+    if (!kAhead) {
+      load(a, xs, p.ldx, row);
+      if (rs) load(b, rs, p.ldr, row);
+    }
+    float f[V][8];
+    unsigned long long sum2 = 0;  // two partial sums
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      unpack8(a[i], f[i]);
+      if (rs) {
+        float t[8];
+        unpack8(b[i], t);
+        add8(f[i], t);
+      }
+      sum2 = squares8(f[i], sum2);
+    }
+    float sum, odd;
+    split_pair(sum2, sum, odd);
+    sum += odd;
+    if (rs) {  // before the next row's loads: h may be x or the residual, whose rows a CTA reads alone
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int col = (i * blockDim.x + tid) * 8;
+        if (col < p.K) {
+          Vec8<T> o;
+          pack8(f[i], o);
+          store8(hs + row * p.ldh + col, o);
+        }
       }
     }
+    if (!kAhead) {
+      load_weight();
+    } else if (rs) {
+      load(a, xs, p.ldx, row + step);
+      load(b, rs, p.ldr, row + step);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int col = (i * blockDim.x + tid) * 8;
-      const bool ok = col < p.K;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f[i][j] = ok ? to_f32(a[i].v[j]) : 0.f;
-        if (rs && ok) f[i][j] += to_f32(r[i].v[j]);
-        sum = fmaf(f[i][j], f[i][j], sum);
-      }
-      if (rs && ok) {
-        Vec8<T> o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o.v[j] = from_f32<T>(f[i][j]);
-        store8(hs + row * p.ldh + col, o);
-      }
+      for (int i = 0; i < V; ++i) a[i] = b[i];
+      load(b, xs, p.ldx, row + 2 * step);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) part[buf][warp] = sum;
-    __syncthreads();  // the other buffer is free: every thread has passed this row's barrier only after reading it
-    sum = lane < warps ? part[buf][lane] : 0.f;
+    // h * weight and the blocks' maxima do not need the row's sum: the root is one factor of a whole row,
+    // and rounding keeps the order of products with it
+    float top[V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float rstd = 1.f / sqrtf(sum / (float)p.K + p.eps);
+    for (int i = 0; i < V; ++i) {
+      float w[8];
+      unpack8(wv[i], w);
+      mul8(f[i], w);  // past the row's end both are 0, and nothing is stored
+      if (p.scale) top[i] = block_top(f[i]);
+    }
+    __syncthreads();  // the other buffer is free: every thread has passed this row's barrier only after reading it
+    sum = part[buf][lane & (wide - 1)];
+    for (int o = wide >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float rstd = rsqrtf(fmaf(sum, inv_k, p.eps));
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int col = (i * blockDim.x + tid) * 8;
       const bool ok = col < p.K;
-      float top = 0.f;
-      if (ok) {
-        const Vec8<W> w = load8(ws + col);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[i][j] = f[i][j] * rstd * to_f32(w.v[j]);
-          top = fmaxf(top, finite_abs(f[i][j]));
-        }
-      }
       uint2 o;
+      mul8(f[i], rstd);
       if (p.scale) {
-        const uint32_t s = scale_byte(half_warp_max(top));
-        const float m = scale_inverse(s);
-        o = make_uint2(e4m3x4(f[i][0] * m, f[i][1] * m, f[i][2] * m, f[i][3] * m),
-                       e4m3x4(f[i][4] * m, f[i][5] * m, f[i][6] * m, f[i][7] * m));
+        const uint32_t s = scale_byte(fmaxf(top[i] * rstd, 0.f));  // a NaN root: no finite value, scale byte 0
+        o = round8(f[i], scale_inverse(s));
         if (ok && (lane & 15) == 0) p.scale[row * p.lds + col / kQBlock] = (uint8_t)s;
       } else {
-        const float m = p.unit;
-        o = make_uint2(s8x4(f[i][0] * m, f[i][1] * m, f[i][2] * m, f[i][3] * m),
-                       s8x4(f[i][4] * m, f[i][5] * m, f[i][6] * m, f[i][7] * m));
+        mul8(f[i], p.unit);
+        o = make_uint2(s8x4(f[i][0], f[i][1], f[i][2], f[i][3]), s8x4(f[i][4], f[i][5], f[i][6], f[i][7]));
       }
       if (ok) *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = o;
     }
@@ -531,7 +689,8 @@ __device__ __forceinline__ void finish_swiglu(const Fp8Params& p, int m, int n, 
   const uint32_t s = scale_byte(top);
   const float r = scale_inverse(s);
   if (ok) {
-    *reinterpret_cast<uint32_t*>(p.q + m * p.ldq + n) = e4m3x4(y[0] * r, y[1] * r, y[2] * r, y[3] * r);
+    *reinterpret_cast<uint32_t*>(p.q + m * p.ldq + n) =
+        e4m3x4(no_infinity(y[0]) * r, no_infinity(y[1]) * r, no_infinity(y[2]) * r, no_infinity(y[3]) * r);
     if ((n & 127) == 0) p.qs[m * p.ldqs + n / kQBlock] = (uint8_t)s;
   }
 }
@@ -553,7 +712,7 @@ __device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&v)
   for (int e = 0; e < 32; ++e) {
     const float y = swiglu_value(__uint_as_float(v[e]), __uint_as_float(u[e]));
     const float top = warp_max(in ? finite_abs(y) : 0.f);
-    v[e] = __float_as_uint(y);
+    v[e] = __float_as_uint(no_infinity(y));
     mine = lane == e ? top : mine;
   }
   tops[lane * 4 + q] = mine;

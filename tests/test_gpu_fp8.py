@@ -93,8 +93,9 @@ def test_quantize_reads_strided_rows_and_writes_only_its_own():
 
 # ---------------------------------------------------------------- norm
 # Relative error of y in fp32: the sum of squares has at most 64 serial additions and 10 levels of tree
-# (74 roundings, all terms positive), halved by the root, then the quotient, the root, its inverse
-# and two products: 45 roundings of 2^-24 at the most.
+# (74 roundings, all terms positive) and the product with 1 / K two more, halved by the root; the
+# reciprocal root is off by two units in the last place (four roundings), then two products: 44
+# roundings of 2^-24 at the most.
 Y_ERR = 45 * 2.0 ** -24
 
 
