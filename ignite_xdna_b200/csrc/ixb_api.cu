@@ -1073,8 +1073,8 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   }
   // Many tokens: persistent pairs.
   for (int mt : {1, 2}) {
-    if ((mode == FP8_SWIGLU && mt == 1) || sms < 2) continue;
-    const int rows = 2 * (mode == FP8_SWIGLU ? 1 : mt);  // weight blocks per tile (of each product)
+    if ((mode == FP8_SWIGLU && mt == 2) || sms < 2) continue;
+    const int rows = mode == FP8_SWIGLU ? 1 : 2 * mt;  // weight blocks per tile (of each product)
     for (int bn = 32; bn <= std::min(256, round_up(M, 32)); bn += 32) {
       const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
       if (mt * bn + sf_cols > 512) break;
@@ -1087,7 +1087,7 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
     }
   }
   const int mt = L.mt, cg = L.cg;
-  const int rows = cg * (mode == FP8_SWIGLU ? 1 : mt);
+  const int rows = mode == FP8_SWIGLU ? 1 : cg * mt;
   p.n_tiles = (nblk + rows - 1) / rows;
   p.m_tiles = (M + p.bn - 1) / p.bn;
   const long long tiles = (long long)p.n_tiles * p.m_tiles;
@@ -1103,7 +1103,7 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   p.stage_bytes = mt * kGemmABlock + p.bn * 128 / cg;
   const int groups = (p.bn + 127) / 128;
   const int sf = kSfSlots * (kSfSpan / 4) * (mt + groups) * kSfAtom;
-  const int stg = cg == 2 && mode == FP8_SWIGLU ? kFp8TopBytes : 0;
+  const int stg = cg == 2 && mode == FP8_SWIGLU ? kFp8SwapBytes + kFp8TopBytes : 0;
   const int fixed = 1024 + sf + stg + kFp8BarBytes;
   // the few-token form leaves room for a second CTA (1 KB of each SM's 228 is the system's, per CTA)
   const int limit = cg == 1 ? kSmemLimit / 2 - 1024 : kSmemLimit;
@@ -1161,7 +1161,7 @@ int launch_fp8(Fp8Launch& L, int mode, cudaStream_t st) {
   Fp8Params& p = L.p;
   p.sf_words = scale_words(p.ws[0], p.ldws[0], p) && (mode == FP8_LINEAR || scale_words(p.ws[1], p.ldws[1], p)) &&
                scale_words(p.xs, p.ldxs, p);
-  if (mode == FP8_SWIGLU) return L.cg == 2 ? launch_fp8_cg<FP8_SWIGLU, 2, 2>(L, st) : launch_fp8_cg<FP8_SWIGLU, 2, 1>(L, st);
+  if (mode == FP8_SWIGLU) return L.cg == 2 ? launch_fp8_cg<FP8_SWIGLU, 1, 2>(L, st) : launch_fp8_cg<FP8_SWIGLU, 2, 1>(L, st);
   if (L.cg == 1) return launch_fp8_cg<FP8_LINEAR, 1, 1>(L, st);
   return L.mt == 1 ? launch_fp8_cg<FP8_LINEAR, 1, 2>(L, st) : launch_fp8_cg<FP8_LINEAR, 2, 2>(L, st);
 }

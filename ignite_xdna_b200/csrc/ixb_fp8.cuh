@@ -471,7 +471,13 @@ constexpr int kFp8FewTokens = 128;                       // tokens per tile of t
 constexpr int kSfSlots = 2;                              // scale images in shared memory
 constexpr int kSfSpan = 16;                              // K-blocks per image: four 32-bit words per row
 constexpr int kSfAtom = 512;                             // bytes of four K-blocks' words of 128 rows
-constexpr int kFp8TopBytes = 2 * 2 * 32 * 4 * 4;         // swiglu epilogue: two groups' two buffers of maxima
+// swiglu pairs: each epilogue warp's two buffers of the peer's columns, and of the maxima; their barriers after
+// the others
+constexpr int kFp8Chunk = 16;
+constexpr int kFp8WarpSwap = kFp8Chunk * 32 * 4;  // one warp's columns: 16 tokens x 32 outputs
+constexpr int kFp8SwapBytes = kFp8Epi * 2 * kFp8WarpSwap;
+constexpr int kFp8TopBytes = 2 * 2 * kFp8Chunk * 4 * 4;
+constexpr int kFp8SwapBar = 384;
 constexpr int kFp8BarBytes = 512;
 enum : int { FP8_LINEAR = 0, FP8_SWIGLU = 1 };
 
@@ -620,8 +626,21 @@ template <int CG>
 __device__ __forceinline__ bool mbar_wait_cg(uint64_t* bar, uint32_t parity) {
   return mbar_poll<CG == 2>(bar, parity);
 }
+// Four words into another CTA's shared memory, counted as 16 bytes on a barrier there: the store itself
+// signals, so no release waits for this thread's earlier global stores.
+__device__ __forceinline__ void st_async4(uint32_t to, const uint32_t* v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+               : "memory");
+}
+// Arrive on a barrier of either CTA: at cluster scope, publishing this thread's writes to the other CTA, and at
+// CTA scope, for what the tensor core reads or has given (TMEM): a release at cluster scope waits for
+// every global store this thread has in flight.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // The next `bytes` (0..4) K-blocks' scale bytes of one row, 4-byte aligned, to a word in shared memory, first
 // block in the low byte, zeros behind.
@@ -701,32 +720,34 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-// Up to 32 tokens' output n of the gate (v) and up (u) products, over a group of four warps that hold a
-// token's 128 outputs: each warp's maxima go through shared memory ([32 tokens][4 warps], two buffers in
-// turn, so one barrier per call), lane c turns token c's into the scale, and every lane rounds.
-__device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&v)[32], const uint32_t (&u)[32], int n, int m0,
-                                               int cols, float* tops, int bar, int q, int lane) {
+// Up to 16 tokens' output n of the gate and up products, over a group of four warps that hold a token's 128
+// outputs: each warp's maxima go through shared memory ([16 tokens][4 warps], two buffers in turn, so
+// one barrier per call), lane c turns token c's into the scale, and every lane rounds. `between` runs
+// once the inputs have been used.
+template <typename F>
+__device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&gate)[kFp8Chunk], const uint32_t (&up)[kFp8Chunk],
+                                               int n, int m0, int cols, float* tops, int bar, int q, int lane, F&& between) {
   const bool in = n < p.N;
   float mine = 0.f;
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    const float y = swiglu_value(__uint_as_float(v[e]), __uint_as_float(u[e]));
+  for (int e = 0; e < kFp8Chunk; ++e) {
+    const float y = swiglu_value(__uint_as_float(gate[e]), __uint_as_float(up[e]));
     const float top = warp_max(in ? finite_abs(y) : 0.f);
-    v[e] = __float_as_uint(no_infinity(y));
+    gate[e] = __float_as_uint(no_infinity(y));
     mine = lane == e ? top : mine;
   }
-  tops[lane * 4 + q] = mine;
+  if (lane < kFp8Chunk) tops[lane * 4 + q] = mine;
+  between();
   group_sync(bar);
-  const float4 t = *reinterpret_cast<const float4*>(tops + lane * 4);
+  const float4 t = *reinterpret_cast<const float4*>(tops + (lane & (kFp8Chunk - 1)) * 4);
   const uint32_t s = scale_byte(fmaxf(fmaxf(t.x, t.y), fmaxf(t.z, t.w)));
-  // the pair's second block may lie wholly past N: it has no scale
-  if (q == 0 && lane < cols && n - lane < p.N) p.qs[(m0 + lane) * p.ldqs + n / kQBlock] = (uint8_t)s;
+  if (q == 0 && lane < cols) p.qs[(m0 + lane) * p.ldqs + n / kQBlock] = (uint8_t)s;
   const float inv = scale_inverse(s);
   uint8_t* o = p.q + m0 * p.ldq + n;
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) {
-    const uint32_t w = e4m3x2(__uint_as_float(v[e]) * __shfl_sync(0xffffffffu, inv, e),
-                              __uint_as_float(v[e + 1]) * __shfl_sync(0xffffffffu, inv, e + 1));
+  for (int e = 0; e < kFp8Chunk; e += 2) {
+    const uint32_t w = e4m3x2(__uint_as_float(gate[e]) * __shfl_sync(0xffffffffu, inv, e),
+                              __uint_as_float(gate[e + 1]) * __shfl_sync(0xffffffffu, inv, e + 1));
     if (in && e < cols) *o = (uint8_t)w;
     o += p.ldq;
     if (in && e + 1 < cols) *o = (uint8_t)(w >> 8);
@@ -734,10 +755,12 @@ __device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&v)
   }
 }
 
-// MODE: FP8_LINEAR or FP8_SWIGLU; MT: blocks of 128 weight rows per tile and CTA (swiglu: 2, gate and
-// up). CG 2: a pair of CTAs shares a tile of twice the weight rows: each holds its own rows' operand,
-// accumulators and epilogue and half of the tokens' operand, and the leader (rank 0) issues the MMAs
-// of both, so each SM fetches half the token bytes per product.
+// MODE: FP8_LINEAR or FP8_SWIGLU; MT: blocks of 128 weight rows per tile and CTA. CG 2: a pair of CTAs
+// shares a tile's tokens: each holds its own rows' operand, accumulators and epilogue and half of the
+// tokens' operand, and the leader (rank 0) issues the MMAs of both, so each SM fetches half the token
+// bytes per product. Swiglu: with CG 1 a CTA has a block of gate rows and the up rows of the same
+// outputs (MT 2); with CG 2 the leader has the gate rows and the other CTA the up rows, so that each has
+// room for two accumulators and the epilogue runs beside the next tile's MMAs.
 // Tiles go through n in groups of p.n_group and through all m within a group, n first: the tiles in work at
 // one time then form a near-square, and what they read (a group's weights, a few rows of x) stays
 // in L2. Through all of n first, 8192 x 4096 x 11008 took 500 us instead of 290.
@@ -749,7 +772,11 @@ __device__ __forceinline__ void tile_at(const Fp8Params& p, int t, int& mt, int&
 }
 template <int MODE, int MT, int CG>
 __device__ __forceinline__ int weight_block(int nt, int pair, int b) {  // 128-row block b of this CTA's part of tile nt
-  return MODE == FP8_SWIGLU ? nt * CG + pair : (nt * CG + pair) * MT + b;
+  return MODE == FP8_SWIGLU ? nt : (nt * CG + pair) * MT + b;
+}
+template <int MODE, int CG>
+__device__ __forceinline__ int weight_source(int pair, int b) {  // which weight it is a block of: 0 (gate), 1 (up)
+  return MODE == FP8_SWIGLU ? (CG == 2 ? pair : b) : 0;
 }
 template <int MODE, int MT, int CG>
 __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
@@ -785,7 +812,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
     // few tokens: this CTA's weights, asked into L2 while the previous kernel drains (a hint; no value is used)
 #pragma unroll
     for (int b = 0; b < MT; ++b) {
-      const int src = MODE == FP8_SWIGLU ? b : 0;
+      const int src = weight_source<MODE, CG>(pair, b);
       const long long row = 128LL * weight_block<MODE, MT, CG>(nt, pair, b) + tid;
       const int k0 = kb0 * 128, k1 = min(p.K, kb1 * 128);
       if (row < p.N) bulk_prefetch_l2(p.w[src] + row * p.ldw[src] + k0, (uint32_t)(k1 - k0));
@@ -806,6 +833,8 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       mbar_init(&acc_empty[b], CG * kFp8Epi);
     }
     mbar_init(done, 1);
+    if (MODE == FP8_SWIGLU && CG == 2)
+      for (int b = 0; b < 2 * kFp8Epi; ++b) mbar_init(reinterpret_cast<uint64_t*>(smem + p.bar_off + kFp8SwapBar) + b, 1);
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.tx) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.tw[0]) : "memory");
@@ -841,7 +870,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
           const uint32_t lead = CG == 2 ? cluster_addr(&full[s], 0) : 0;
 #pragma unroll
           for (int b = 0; b < MT; ++b) {
-            const CUtensorMap* tw = &p.tw[MODE == FP8_SWIGLU ? b : 0];
+            const CUtensorMap* tw = &p.tw[weight_source<MODE, CG>(pair, b)];
             const int row = weight_block<MODE, MT, CG>(nt, pair, b) * 128;
             if (CG == 2) tma_load_2d_pair(st + b * kGemmABlock, tw, kb * 128, row, lead);
             else tma_load_2d(st + b * kGemmABlock, tw, kb * 128, row, &full[s]);
@@ -872,7 +901,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       bool in[MT + kXRows];
 #pragma unroll
       for (int b = 0; b < MT; ++b) {
-        const int src = MODE == FP8_SWIGLU ? b : 0;
+        const int src = weight_source<MODE, CG>(pair, b);
         const long long r = weight_block<MODE, MT, CG>(nt, pair, b);
         in[b] = r * 128 < p.N;
         row[b] = p.ws[src] + (in[b] ? r : 0) * p.ldws[src];
@@ -1016,50 +1045,36 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
     }
   } else if constexpr (CG == 2) {
     // ------------------------------------------------------------ epilogue
-    // A warp reads 32 columns of its TMEM lane quarter at a time (a lane holds one output n of 32
-    // tokens) and stores each token's 32 outputs as one run; the two groups of four warps take
-    // alternate columns. The accumulator is handed back once its last columns are in registers.
-    // After a wait that gave up every warp runs on without work: all reach every barrier.
+    // A lane holds one output n of a run of tokens, a warp 32 outputs and a group of four warps 128, and
+    // each token's outputs are stored as one run; the two groups take alternate runs of tokens. The
+    // accumulator is handed back once its last columns are in registers. After a wait that gave up
+    // every warp runs on without work: all reach every barrier.
     const int q = warp & 3, g = warp >> 2;
-    const int nch = (p.bn + 31) / 32;
-    const int items = MODE == FP8_SWIGLU ? nch : MT * nch;
-    float* tops = reinterpret_cast<float*>(smem + p.stg_off) + g * (2 * 32 * 4);
-    int acc = 0, buf = 0;
+    int acc = 0;
     uint32_t aph = 0;
     bool ok = true;
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (CG == 2) mbar_arrive_cluster(cluster_addr(&acc_empty[acc], 0));
-        else mbar_arrive(&acc_empty[acc]);
-      }
+      if (lane == 0) mbar_arrive_remote(cluster_addr(&acc_empty[acc], 0));
     };
-    for (int t = tile0; t < tiles; t += tstep) {
-      ok = mbar_poll(&acc_full[acc], aph) && ok;
-      tc_fence_after();
-      int mt, nt;
-      tile_at(p, t, mt, nt);
-      const uint32_t base = tmem + acc * p.acc_cols + ((uint32_t)(q * 32) << 16);
-      if (g >= items) release();
-      for (int i = g; i < items; i += kFp8Epi / 4) {
-        const int blk = MODE == FP8_SWIGLU ? 0 : i / nch, c = (i - blk * nch) * 32;
-        const bool both = c + 16 < p.bn;  // bn is a multiple of 16
-        const int n = weight_block<MODE, MT, CG>(nt, pair, blk) * 128 + q * 32 + lane;
-        const int m0 = mt * p.bn + c;
-        const int cols = ok ? min(both ? 32 : 16, p.M - m0) : 0;  // tokens of this run
-        uint32_t v[32];
-        tmem_ld16(base + blk * p.bn + c, reinterpret_cast<uint32_t(&)[16]>(v[0]));
-        if (both) tmem_ld16(base + blk * p.bn + c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
-        if constexpr (MODE == FP8_SWIGLU) {
-          uint32_t u[32];
-          tmem_ld16(base + p.bn + c, reinterpret_cast<uint32_t(&)[16]>(u[0]));
-          if (both) tmem_ld16(base + p.bn + c + 16, reinterpret_cast<uint32_t(&)[16]>(u[16]));
-          tmem_ld_wait();
-          if (i + kFp8Epi / 4 >= items) release();
-          swiglu_columns(p, v, u, n, m0, cols, tops + buf * (32 * 4), 1 + g, q, lane);
-          buf ^= 1;
-        } else {
+    if constexpr (MODE == FP8_LINEAR) {
+      const int nch = (p.bn + 31) / 32, items = MT * nch;
+      for (int t = tile0; t < tiles; t += tstep) {
+        ok = mbar_poll(&acc_full[acc], aph) && ok;
+        tc_fence_after();
+        int mt, nt;
+        tile_at(p, t, mt, nt);
+        const uint32_t base = tmem + acc * p.acc_cols + ((uint32_t)(q * 32) << 16);
+        if (g >= items) release();
+        for (int i = g; i < items; i += kFp8Epi / 4) {
+          const int blk = i / nch, c = (i - blk * nch) * 32;  // bn is a multiple of 32
+          const int n = weight_block<MODE, MT, CG>(nt, pair, blk) * 128 + q * 32 + lane;
+          const int m0 = mt * p.bn + c;
+          const int cols = ok ? min(32, p.M - m0) : 0;  // tokens of this run
+          uint32_t v[32];
+          tmem_ld16(base + blk * p.bn + c, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+          tmem_ld16(base + blk * p.bn + c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
           tmem_ld_wait();
           if (i + kFp8Epi / 4 >= items) release();
           if (n < p.N) {
@@ -1068,10 +1083,71 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             else store_columns(static_cast<float*>(p.out), p.ldo, v, n, m0, cols);
           }
         }
+        if (++acc == p.nacc) {
+          acc = 0;
+          aph ^= 1;
+        }
       }
-      if (++acc == p.nacc) {
-        acc = 0;
-        aph ^= 1;
+    } else {
+      // Of each two runs of 16 tokens the leader finishes the first and the other CTA the second: a warp sends
+      // the peer's warp of the same lanes its product's columns of the peer's run, and takes the peer's
+      // columns of its own run. Two buffers, and no message that says one is free: a warp sends run k
+      // only after it has used the peer's run k - 1, which the peer sent after it had used this
+      // warp's run k - 2. (With releases in place of st.async each exchange waited for the rounded
+      // values' global stores: 23,000 cycles per tile of 224 tokens.)
+      uint8_t* recv = smem + p.stg_off + warp * (2 * kFp8WarpSwap) + lane * 16;  // [4 tokens each][lane][4]
+      float* tops = reinterpret_cast<float*>(smem + p.stg_off + kFp8SwapBytes) + g * (2 * kFp8Chunk * 4);
+      uint64_t* swap = reinterpret_cast<uint64_t*>(smem + p.bar_off + kFp8SwapBar) + 2 * warp;  // the peer's columns have come
+      const uint32_t peer_recv = cluster_addr(recv, 1 - pair), peer_swap = cluster_addr(swap, 1 - pair);
+      const int pairs = p.bn / (2 * kFp8Chunk);
+      int sbuf = 0, rbuf = 0;
+      uint32_t rph = 0;
+      for (int t = tile0; t < tiles; t += tstep) {
+        ok = mbar_poll(&acc_full[acc], aph) && ok;
+        tc_fence_after();
+        int mt, nt;
+        tile_at(p, t, mt, nt);
+        const uint32_t base = tmem + acc * p.acc_cols + ((uint32_t)(q * 32) << 16);
+        const int n = nt * 128 + q * 32 + lane;
+        auto send = [&](int i) {
+          uint32_t u[kFp8Chunk];
+          tmem_ld16(base + i * 2 * kFp8Chunk + (1 - pair) * kFp8Chunk, u);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < kFp8Chunk; e += 4) st_async4(peer_recv + sbuf * kFp8WarpSwap + e * (32 * 4), u + e, peer_swap + 8 * sbuf);
+          sbuf ^= 1;
+        };
+        if (g >= pairs) release();
+        else send(g);
+        for (int i = g; i < pairs; i += kFp8Epi / 4) {
+          uint32_t v[kFp8Chunk], u[kFp8Chunk];
+          tmem_ld16(base + i * 2 * kFp8Chunk + pair * kFp8Chunk, v);
+          if (lane == 0) mbar_arrive_expect_tx(&swap[rbuf], kFp8WarpSwap);
+          ok = mbar_poll<true>(&swap[rbuf], rph) && ok;
+#pragma unroll
+          for (int e = 0; e < kFp8Chunk; e += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(recv + rbuf * kFp8WarpSwap + e * (32 * 4));
+            u[e] = w.x;
+            u[e + 1] = w.y;
+            u[e + 2] = w.z;
+            u[e + 3] = w.w;
+          }
+          tmem_ld_wait();
+          const int m0 = mt * p.bn + i * 2 * kFp8Chunk + pair * kFp8Chunk, cols = ok ? min(kFp8Chunk, p.M - m0) : 0;
+          float* part = tops + rbuf * (kFp8Chunk * 4);
+          auto next = [&] {
+            if (i + kFp8Epi / 4 < pairs) send(i + kFp8Epi / 4);
+            else release();
+          };
+          if (pair == 0) swiglu_columns(p, v, u, n, m0, cols, part, 1 + g, q, lane, next);
+          else swiglu_columns(p, u, v, n, m0, cols, part, 1 + g, q, lane, next);
+          rbuf ^= 1;
+          if (rbuf == 0) rph ^= 1;
+        }
+        if (++acc == p.nacc) {
+          acc = 0;
+          aph ^= 1;
+        }
       }
     }
   } else {

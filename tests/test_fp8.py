@@ -29,7 +29,7 @@ def test_plans_fit_the_hardware(swiglu):
                 groups = -(-p["bn"] // 128)
                 assert p["bn"] % 16 == 0 and 16 <= p["bn"] <= 256 and p["mt"] in (1, 2)
                 assert p["cg"] in (1, 2) and p["bn"] % (16 * p["cg"]) == 0 and (p["cg"] == 1 or p["split"] == 1)
-                assert p["m_tiles"] * p["bn"] >= M and p["n_tiles"] * 128 * p["cg"] * (1 if swiglu else p["mt"]) >= N
+                assert p["m_tiles"] * p["bn"] >= M and p["n_tiles"] * 128 * (1 if swiglu else p["cg"] * p["mt"]) >= N
                 assert p["kblocks"] * 128 >= K and p["stages"] >= 1 and p["smem"] <= 227 * 1024
                 assert p["nacc"] * p["mt"] * p["bn"] + 8 * (p["mt"] + groups) <= p["tmem"] <= 512
                 assert p["tmem"] & (p["tmem"] - 1) == 0
