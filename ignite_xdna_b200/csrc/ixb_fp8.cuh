@@ -426,7 +426,9 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
     __syncthreads();  // the other buffer is free: every thread has passed this row's barrier only after reading it
     sum = part[buf][lane & (wide - 1)];
     for (int o = wide >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float rstd = rsqrtf(fmaf(sum, inv_k, p.eps));
+    const float mean = fmaf(sum, inv_k, p.eps);
+    float rstd = rsqrtf(mean);
+    if (mean <= FLT_MAX) rstd *= fmaf(-0.5f * mean * rstd, rstd, 1.5f);  // a Newton step: two units in the last place to one
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int col = (i * blockDim.x + tid) * 8;
@@ -460,9 +462,10 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
 //
 // Two forms. Few tokens (CG 1): tiles of at most 128 tokens, one per CTA or cluster; a cluster of up to
 // four CTAs shares a tile along K and adds its 32-bit parts in rank order over distributed shared
-// memory; shared memory and registers leave room for two CTAs per SM, so the next kernel's start,
-// and its prefetch of its weights into L2, overlap this one's end. Many tokens (CG 2): persistent
-// pairs of CTAs.
+// memory; shared memory and registers leave room for two CTAs per SM, so the next kernel's start
+// overlaps this one's end. (Asking the weights into L2 before waiting for the previous kernel, as the
+// W4A8 GEMV does, gained nothing: 18.4 us without and 20.0 with it for 8 x 11008 x 4096 gate/up.) Many
+// tokens (CG 2): persistent pairs of CTAs.
 constexpr int kFp8Epi = 8;                               // epilogue warps, two groups of four
 constexpr int kFp8Threads = 32 * (kFp8Epi + 3);          // + TMA producer, MMA issuer, scale gatherer
 constexpr int kFp8MaxStages = 12;
@@ -493,8 +496,6 @@ struct Fp8Params {
   const uint8_t* ws[2];
   long long ldxs, ldws[2];
   int sf_words;  // every scale word is 4-byte aligned
-  const uint8_t* w[2];  // the weights, for the L2 prefetch of few tokens; null: none
-  long long ldw[2];
   int out_type;
   void* out;            // linear
   long long ldo;
@@ -695,8 +696,17 @@ __device__ __forceinline__ void finish_linear(const Fp8Params& p, int m, int n, 
   else if (p.out_type == FT_F16) store_out4(static_cast<__half*>(p.out) + m * p.ldo, n, p.N, v);
   else store_out4(static_cast<float*>(p.out) + m * p.ldo, n, p.N, v);
 }
-// silu(g) * u. The quotient's and the exponential's few units in the last place are far inside e4m3's 2^-4.
-__device__ __forceinline__ float swiglu_value(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// g / (1 + exp(-g)) * u within a few units in the last place, for a value next to a rounding or scale border
+// should fall on the side that exact arithmetic puts it. expf is CUDA's; the reciprocal is the
+// hardware's with one Newton step, where that is finite (past 2^100 the quotient is far below any
+// other output's).
+__device__ __forceinline__ float swiglu_value(float g, float u) {
+  const float d = 1.f + expf(-g);
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(d));
+  r = d < 0x1p100f ? fmaf(fmaf(-d, r, 1.f), r, r) : r;
+  return g * r * u;
+}
 __device__ __forceinline__ void finish_swiglu(const Fp8Params& p, int m, int n, float4 g, float4 u) {
   float y[4] = {swiglu_value(g.x, u.x), swiglu_value(g.y, u.y), swiglu_value(g.z, u.z), swiglu_value(g.w, u.w)};
   const bool ok = n < p.N;  // N is a multiple of 16, n of 4
@@ -806,18 +816,6 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   const int sf_quad = (MT + sfb_groups) * kSfAtom;  // four K-blocks' images
 
   grid_dep_launch();
-  if (p.w[0] && tid < 128) {
-    int mt, nt;
-    tile_at(p, tile0, mt, nt);
-    // few tokens: this CTA's weights, asked into L2 while the previous kernel drains (a hint; no value is used)
-#pragma unroll
-    for (int b = 0; b < MT; ++b) {
-      const int src = weight_source<MODE, CG>(pair, b);
-      const long long row = 128LL * weight_block<MODE, MT, CG>(nt, pair, b) + tid;
-      const int k0 = kb0 * 128, k1 = min(p.K, kb1 * 128);
-      if (row < p.N) bulk_prefetch_l2(p.w[src] + row * p.ldw[src] + k0, (uint32_t)(k1 - k0));
-    }
-  }
   if (warp == MW) tmem_alloc_cg<CG>(tmem_slot, p.tmem_cols);
   if (tid == PW * 32) {
     for (int s = 0; s < S; ++s) {
@@ -963,9 +961,8 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   } else if (warp == MW) {
     // ------------------------------------------------------------ MMA issuer
     // The tensor core's queue holds little more than the MMA it works on, so what this warp does between
-    // two K-blocks has to fit beside the last MMAs of the first: descriptors advance by additions, the
-    // next stage's barrier is looked at while the MMAs run, and a K tail costs no branch (the TMA's
-    // zeros fill it).
+    // two K-blocks has to fit beside the last MMAs of the first: descriptors advance by additions, and a
+    // K tail costs no branch (the TMA's zeros fill it).
     if (pair == 0) {
       int s = 0, acc = 0, ss = 0;
       uint32_t ph = 0, aph = 0, sph = 0, sfbuf = 0;
@@ -974,7 +971,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       const uint32_t dstep = (uint32_t)p.stage_bytes >> 4;  // descriptors count in 16 bytes
       const uint64_t ad0 = umma_desc_sw128(smem_u32(smem));
       uint64_t ad = ad0;
-      bool ready = false;
+      constexpr uint32_t kNextScale = (1u << 29) | (1u << 4);  // the next byte of both scale words
       for (int t = tile0; ok && t < tiles; t += tstep) {
         if (!warp_all(mbar_wait_cg<CG>(&acc_empty[acc], aph ^ 1))) break;
         tc_fence_after();
@@ -995,33 +992,44 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             sfbuf ^= 1;
             uint32_t idesc = p.idesc;
             const int n = min(4, end - kq);
-            for (int i = 0; i < n; ++i) {
-              if (!ready && !warp_all(mbar_poll(&full[s], ph))) {
+            for (int i = 0; i < n;) {
+              // two stages at a time where the second has landed too: one look, one election, one turn of the loop
+              const int s1 = s + 1 == S ? 0 : s + 1;
+              const bool t0 = mbar_test(&full[s], ph), t1 = mbar_test(&full[s1], ph ^ (s1 == 0 ? 1u : 0u));
+              if (!warp_all(t0) && !warp_all(mbar_poll(&full[s], ph))) {
                 ok = false;
                 break;
               }
+              const bool both = warp_all(t1) && i + 1 < n && S > 1;
               tc_fence_after();
-              const int s1 = s + 1 == S ? 0 : s + 1;
-              const bool next = mbar_test(&full[s1], ph ^ (s1 == 0 ? 1u : 0u));  // looked at while the MMAs are issued
               if (elect_one()) {
-                const uint64_t bd = ad + MT * (kGemmABlock >> 4);
+                auto issue = [&](uint64_t a, uint32_t id, uint32_t first) {
+                  const uint64_t bd = a + MT * (kGemmABlock >> 4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                  for (int j = 0; j < 4; ++j)
 #pragma unroll
-                  for (int b = 0; b < MT; ++b)
-                    umma_mxf8<CG>(d0 + b * p.bn, ad + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, idesc, sf + 4 * b, sf + 4 * MT,
-                                  j ? 1u : accumulate);
+                    for (int b = 0; b < MT; ++b)
+                      umma_mxf8<CG>(d0 + b * p.bn, a + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, id, sf + 4 * b, sf + 4 * MT,
+                                    j ? 1u : first);
+                };
+                issue(ad, idesc, accumulate);
                 umma_commit_cg<CG>(&empty[s]);
+                if (both) {
+                  issue(s1 == 0 ? ad0 : ad + dstep, idesc + kNextScale, 1u);
+                  umma_commit_cg<CG>(&empty[s1]);
+                }
               }
-              ready = warp_all(next);
-              idesc += (1u << 29) | (1u << 4);  // the next byte of both scale words
               accumulate = 1;
               issued = true;
-              ad += dstep;
-              s = s1;
-              if (s == 0) {
+              const int step = both ? 2 : 1;
+              i += step;
+              idesc += both ? 2 * kNextScale : kNextScale;
+              s += step;
+              ad += both ? 2 * dstep : dstep;
+              if (s >= S) {
+                s -= S;
                 ph ^= 1;
-                ad = ad0;
+                ad = ad0 + s * dstep;
               }
             }
           }
