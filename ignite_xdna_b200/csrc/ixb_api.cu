@@ -1055,8 +1055,8 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
     p.kb_split = kbs;
     p.nacc = nacc;
   };
-  // The estimates are microseconds, fitted to 849 timed plans of 54 shapes (1 to 8192 tokens): the plan
-  // they choose was 1.6 % slower than the fastest on average.
+  // The estimates are microseconds, fitted to 900 timed plans of 66 shapes (1 to 8192 tokens), the large ones
+  // under the power cap: the plan they choose was 1 % slower than the fastest on average.
   // Few tokens: a CTA per tile and part of K, two of them on an SM at a time, which hide one another's
   // latency (a K-block takes a CTA 0.38 us alone) until the operands' arrival or the MMAs bound both.
   {
@@ -1066,7 +1066,8 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
       const int stage = mt * kGemmABlock + bn * 128;
       for (int split = 1; split <= kFp8MaxSplit; ++split) {
         const int kbs = (p.kblocks + split - 1) / split;
-        if (split > 1 && ((split - 1) * kbs >= p.kblocks || tiles * split > 2LL * sms)) break;
+        // nine tenths of the places, for a cluster's CTAs lie in one group of SMs and the last places stay empty
+        if (split > 1 && ((split - 1) * kbs >= p.kblocks || tiles * split > 9LL * sms / 5)) break;
         const long long per_sm = (tiles * split + sms - 1) / sms;
         auto round = [&](int ctas) {
           return kbs * std::max(0.384, ctas * std::max(mt * bn * 0.00207, stage * 7.8e-6)) + ctas * mt * bn * 0.025;
@@ -1086,8 +1087,8 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
       const long long tiles = (long long)((nblk + rows - 1) / rows) * ((M + bn - 1) / bn);
       const long long waves = (tiles + sms / 2 - 1) / (sms / 2);
       const bool two = waves > 1 && 2 * mt * bn + sf_cols <= 512;
-      const double kb = std::max(mt * bn * 0.000965 + 0.135, 0.2825), epi = mt * bn * 0.00828;
-      take(4.06 + waves * p.kblocks * kb + (two ? 1 : waves) * epi, 2, mt, bn, 1, p.kblocks, two ? 2 : 1);
+      const double tile = p.kblocks * std::max(mt * bn * 0.001106 + 0.0874, 0.308) + 0.824, epi = mt * bn * 0.01;
+      take(2.36 + (two ? waves * std::max(tile, epi) + epi : waves * (tile + epi)), 2, mt, bn, 1, p.kblocks, two ? 2 : 1);
     }
   }
   const int mt = L.mt, cg = L.cg;

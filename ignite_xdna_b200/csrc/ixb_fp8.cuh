@@ -971,7 +971,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       const uint32_t dstep = (uint32_t)p.stage_bytes >> 4;  // descriptors count in 16 bytes
       const uint64_t ad0 = umma_desc_sw128(smem_u32(smem));
       uint64_t ad = ad0;
-      constexpr uint32_t kNextScale = (1u << 29) | (1u << 4);  // the next byte of both scale words
+      bool ready = false;
       for (int t = tile0; ok && t < tiles; t += tstep) {
         if (!warp_all(mbar_wait_cg<CG>(&acc_empty[acc], aph ^ 1))) break;
         tc_fence_after();
@@ -992,44 +992,33 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             sfbuf ^= 1;
             uint32_t idesc = p.idesc;
             const int n = min(4, end - kq);
-            for (int i = 0; i < n;) {
-              // two stages at a time where the second has landed too: one look, one election, one turn of the loop
-              const int s1 = s + 1 == S ? 0 : s + 1;
-              const bool t0 = mbar_test(&full[s], ph), t1 = mbar_test(&full[s1], ph ^ (s1 == 0 ? 1u : 0u));
-              if (!warp_all(t0) && !warp_all(mbar_poll(&full[s], ph))) {
+            for (int i = 0; i < n; ++i) {
+              if (!ready && !warp_all(mbar_poll(&full[s], ph))) {
                 ok = false;
                 break;
               }
-              const bool both = warp_all(t1) && i + 1 < n && S > 1;
               tc_fence_after();
+              const int s1 = s + 1 == S ? 0 : s + 1;
+              const bool next = mbar_test(&full[s1], ph ^ (s1 == 0 ? 1u : 0u));  // looked at while the MMAs are issued
               if (elect_one()) {
-                auto issue = [&](uint64_t a, uint32_t id, uint32_t first) {
-                  const uint64_t bd = a + MT * (kGemmABlock >> 4);
+                const uint64_t bd = ad + MT * (kGemmABlock >> 4);
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int b = 0; b < MT; ++b)
-                      umma_mxf8<CG>(d0 + b * p.bn, a + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, id, sf + 4 * b, sf + 4 * MT,
-                                    j ? 1u : first);
-                };
-                issue(ad, idesc, accumulate);
+                  for (int b = 0; b < MT; ++b)
+                    umma_mxf8<CG>(d0 + b * p.bn, ad + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, idesc, sf + 4 * b, sf + 4 * MT,
+                                  j ? 1u : accumulate);
                 umma_commit_cg<CG>(&empty[s]);
-                if (both) {
-                  issue(s1 == 0 ? ad0 : ad + dstep, idesc + kNextScale, 1u);
-                  umma_commit_cg<CG>(&empty[s1]);
-                }
               }
+              ready = warp_all(next);
+              idesc += (1u << 29) | (1u << 4);  // the next byte of both scale words
               accumulate = 1;
               issued = true;
-              const int step = both ? 2 : 1;
-              i += step;
-              idesc += both ? 2 * kNextScale : kNextScale;
-              s += step;
-              ad += both ? 2 * dstep : dstep;
-              if (s >= S) {
-                s -= S;
+              ad += dstep;
+              s = s1;
+              if (s == 0) {
                 ph ^= 1;
-                ad = ad0 + s * dstep;
+                ad = ad0;
               }
             }
           }
