@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
 // ---------------------------------------------------------------- products
 // tcgen05.mma kind::mxf8f6f4 with block scales. The weight rows are the MMA's M (128 rows: one
 // scale for the whole block), the tokens its N, so a single token costs a 16-column MMA and a
-// long prompt a 240-column one in the same kernel. Each MMA takes 32 of K; the four of a
+// long prompt a 224-column one in the same kernel. Each MMA takes 32 of K; the four of a
 // 128-block use the same scale byte. A tile is MT blocks of 128 weight rows (swiglu: one block
 // of gate rows and the up rows of the same outputs) by bn tokens.
 //
@@ -461,15 +461,19 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
 // tcgen05.cp (32x128b, warpx4) brings that into TMEM, in order before the MMAs that read it.
 //
 // Two forms. Few tokens (CG 1): tiles of at most 128 tokens, one per CTA or cluster; a cluster of up to
-// four CTAs shares a tile along K and adds its 32-bit parts in rank order over distributed shared
+// eight CTAs shares a tile along K and adds its 32-bit parts in rank order over distributed shared
 // memory; shared memory and registers leave room for two CTAs per SM, so the next kernel's start
-// overlaps this one's end. (Asking the weights into L2 before waiting for the previous kernel, as the
+// overlaps this one's end. HBM bounds it (the weights are read once), with ~3 us of start and end:
+// 1 x 4096 x 4096 5.8 us, 23 x 4096 x 11008 11.9 us (3.8 TB/s), 8 x 11008 x 4096 gate/up 18 us (5 TB/s). (Asking the weights into L2 before waiting for the previous kernel, as the
 // W4A8 GEMV does, gained nothing: 18.4 us without and 20.0 with it for 8 x 11008 x 4096 gate/up.) Many
-// tokens (CG 2): persistent pairs of CTAs.
+// tokens (CG 2): persistent pairs of CTAs, tiles of 256 weight rows x 224 tokens with two accumulators
+// (or 512 rows and one, where that is one round). The tensor cores bound it, and in a long run the
+// board's 1000 W: 8192 x 11008 x 4096 takes 256 us (2.9 PFLOP/s) in a burst and 301 us at the ~1.05 GHz
+// that the cap leaves, where the MMAs alone would take 300.
 constexpr int kFp8Epi = 8;                               // epilogue warps, two groups of four
 constexpr int kFp8Threads = 32 * (kFp8Epi + 3);          // + TMA producer, MMA issuer, scale gatherer
 constexpr int kFp8MaxStages = 12;
-constexpr int kFp8MaxSplit = 4;                          // CTAs that share a tile along K (eight took twice as long to start)
+constexpr int kFp8MaxSplit = 8;                          // CTAs that share a tile along K: a portable cluster
 constexpr int kFp8FewTokens = 128;                       // tokens per tile of the split form
 constexpr int kSfSlots = 2;                              // scale images in shared memory
 constexpr int kSfSpan = 16;                              // K-blocks per image: four 32-bit words per row
@@ -575,8 +579,8 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* t
       "l"(tm), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// A bounded wait that polls: a wait with a suspend hint takes about a microsecond to wake, and every
-// K-block hands a stage from the TMA to the tensor core and back. Same limit and flag as mbar_wait.
+// A bounded wait without a suspend hint: every K-block hands a stage from the TMA to the tensor core and back,
+// and waking from a long sleep is on that way. Same limit and flag as mbar_wait.
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -765,15 +769,9 @@ __device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&ga
   }
 }
 
-// MODE: FP8_LINEAR or FP8_SWIGLU; MT: blocks of 128 weight rows per tile and CTA. CG 2: a pair of CTAs
-// shares a tile's tokens: each holds its own rows' operand, accumulators and epilogue and half of the
-// tokens' operand, and the leader (rank 0) issues the MMAs of both, so each SM fetches half the token
-// bytes per product. Swiglu: with CG 1 a CTA has a block of gate rows and the up rows of the same
-// outputs (MT 2); with CG 2 the leader has the gate rows and the other CTA the up rows, so that each has
-// room for two accumulators and the epilogue runs beside the next tile's MMAs.
 // Tiles go through n in groups of p.n_group and through all m within a group, n first: the tiles in work at
-// one time then form a near-square, and what they read (a group's weights, a few rows of x) stays
-// in L2. Through all of n first, 8192 x 4096 x 11008 took 500 us instead of 290.
+// one time then form a near-square, and what they read (a group's weights, a few rows of x) is read
+// from L2 by as few as can be (8192 x 11008 x 4096: 270 us, through all of n first 279).
 __device__ __forceinline__ void tile_at(const Fp8Params& p, int t, int& mt, int& nt) {
   const int per = p.n_group * p.m_tiles, g = t / per, r = t - g * per;
   const int size = min(p.n_group, p.n_tiles - g * p.n_group);
@@ -788,6 +786,12 @@ template <int MODE, int CG>
 __device__ __forceinline__ int weight_source(int pair, int b) {  // which weight it is a block of: 0 (gate), 1 (up)
   return MODE == FP8_SWIGLU ? (CG == 2 ? pair : b) : 0;
 }
+// MODE: FP8_LINEAR or FP8_SWIGLU; MT: blocks of 128 weight rows per tile and CTA. CG 2: a pair of CTAs
+// shares a tile's tokens: each holds its own rows' operand, accumulators and epilogue and half of the
+// tokens' operand, and the leader (rank 0) issues the MMAs of both, so each SM fetches half the token
+// bytes per product. Swiglu: with CG 1 a CTA has a block of gate rows and the up rows of the same
+// outputs (MT 2); with CG 2 the leader has the gate rows and the other CTA the up rows, so that each has
+// room for two accumulators and the epilogue runs beside the next tile's MMAs.
 template <int MODE, int MT, int CG>
 __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(const __grid_constant__ Fp8Params p) {
   constexpr int PW = kFp8Epi, MW = kFp8Epi + 1, SW = kFp8Epi + 2;
@@ -849,8 +853,8 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   if (warp == PW) {
     // ------------------------------------------------------------ TMA producer
     // This warp's and the MMA warp's loops run in all lanes and one elected lane issues, so addresses and
-    // descriptors stay in uniform registers: a loop inside `if (lane == 0)` cost about 900 cycles
-    // per K-block in moving them there, whatever the tile.
+    // descriptors stay in uniform registers (with the loops inside `if (lane == 0)` 8192 x 11008 x 4096
+    // took 372 us instead of 318, at that time).
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
@@ -1179,19 +1183,21 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
         float4 v[MT];
 #pragma unroll
         for (int b = 0; b < MT; ++b) {
-          float4 part[kFp8MaxSplit];
+          v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int r0 = 0; r0 < p.split; r0 += 4) {  // four loads in flight
+            float4 part[4];
 #pragma unroll
-          for (int r = 0; r < kFp8MaxSplit; ++r)
-            if (r < p.split) part[r] = ld_cluster_f4(cluster_addr(smem + ((b * p.bn + c) * 128 + lane * 4) * 4, r));
-          v[b] = part[0];
+            for (int r = 0; r < 4; ++r)
+              if (r0 + r < p.split) part[r] = ld_cluster_f4(cluster_addr(smem + ((b * p.bn + c) * 128 + lane * 4) * 4, r0 + r));
 #pragma unroll
-          for (int r = 1; r < kFp8MaxSplit; ++r)
-            if (r < p.split) {
-              v[b].x += part[r].x;
-              v[b].y += part[r].y;
-              v[b].z += part[r].z;
-              v[b].w += part[r].w;
-            }
+            for (int r = 0; r < 4; ++r)
+              if (r0 + r < p.split) {
+                v[b].x += part[r].x;
+                v[b].y += part[r].y;
+                v[b].z += part[r].z;
+                v[b].w += part[r].w;
+              }
+          }
         }
         if constexpr (MODE == FP8_SWIGLU) finish_swiglu(p, m, nt * 128 + lane * 4, v[0], v[1]);
         else finish_linear(p, m, nt * 128 + lane * 4, v[0]);

@@ -296,8 +296,11 @@ int ixb_u8i4_gemm_i32(const uint8_t* a, const uint8_t* image, int32_t* out, int 
  * [ceil(N/128)][ceil(K/128)]; the last block of a row or column may be short. Values are the OCP e4m3
  * (largest 448, no infinities). Strides (ld...) are in elements between rows. Device pointers;
  * matrices 16-byte aligned with row strides that are multiples of 16 bytes (scales and the output of
- * ixb_fp8_linear: any). K a multiple of 16, any M (0 returns at once). Enqueued on `stream`, with
- * programmatic dependent launch as ixb_w4a8_gemv; capture-safe, no allocation, no workspace. */
+ * ixb_fp8_linear: any). K a multiple of 16, M from 0 (returns at once) to 2^30. Outputs overlap no
+ * input but where said. Enqueued on `stream` with programmatic dependent launch: each kernel lets the
+ * next one start early and itself waits for the previous one before it reads or writes memory.
+ * Capture-safe, no allocation, no workspace. A kernel whose bounded wait gave up raises the device flag
+ * (ixb_device_error). */
 #define IXB_BF16 0
 #define IXB_F16 1
 #define IXB_F32 2

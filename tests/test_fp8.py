@@ -44,7 +44,7 @@ def test_plans_fit_the_hardware(swiglu):
 def test_plan_refuses_bad_sizes():
     info = (C.c_int32 * 13)()
     lib = L.load()
-    for M, N, K in [(0, 16, 16), (-1, 16, 16), (16, 0, 16), (16, 16, 8), (16, 16, 24), (16, 16, 0), (1, 1 << 25, 16),
+    for M, N, K in [(0, 16, 16), (-1, 16, 16), ((1 << 30) + 1, 16, 16), (16, 0, 16), (16, 16, 8), (16, 16, 24), (16, 16, 0), (1, 1 << 25, 16),
                     (1, 16, 65552)]:
         assert lib.ixb_fp8_plan_info(M, N, K, 0, info, 13) == L.IXB_ERR_INVALID, (M, N, K)
     assert lib.ixb_fp8_plan_info(16, 16, 16, 0, info, 12) == L.IXB_ERR_INVALID

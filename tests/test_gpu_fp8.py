@@ -174,6 +174,24 @@ def test_norm_in_place(M):
         assert torch.equal(at, h0) and same_bits(q, q0) and same_bits(s, s0)
 
 
+@pytest.mark.parametrize("M,K", [(1, 144), (3, 2064), (400, 272), (310, 16400)])
+def test_norm_writes_only_its_own(M, K):
+    x = randn(M, K, seed=1, dtype=torch.bfloat16)
+    r = randn(M, K, seed=2, dtype=torch.bfloat16)
+    w = randn(K, seed=3, dtype=torch.bfloat16)
+    q, s, h = fp8.rmsnorm_quant(x, w, residual=r)
+    nb = -(-K // 128)
+    qb = torch.full((M + 1, K + 48), 0x55, dtype=torch.uint8, device="cuda")
+    sb = torch.full((M + 1, nb + 2), 0x55, dtype=torch.uint8, device="cuda")
+    hb = torch.full((M + 1, K + 24), 7.0, dtype=torch.bfloat16, device="cuda")
+    L.check(L.load().ixb_rmsnorm_quant(x.data_ptr(), K, r.data_ptr(), K, w.data_ptr(), L.BF16, L.BF16, M, K, 1e-6, 0, hb.data_ptr(),
+                                       K + 24, qb.data_ptr(), K + 48, sb.data_ptr(), nb + 2, None))
+    settle()
+    assert torch.equal(qb[:M, :K], q.view(torch.uint8)) and torch.equal(sb[:M, :nb], s.view(torch.uint8)) and torch.equal(hb[:M, :K], h)
+    assert (qb[:, K:] == 0x55).all() and (qb[M] == 0x55).all() and (sb[:, nb:] == 0x55).all() and (sb[M] == 0x55).all()
+    assert (hb[:, K:] == 7).all() and (hb[M] == 7).all()
+
+
 # ---------------------------------------------------------------- product
 def slack(K, total):
     """Error of an fp32 sum of K exact products whose absolute values add up to `total`, each addition
@@ -346,6 +364,39 @@ def test_linear_swiglu_large_gates_and_nan():
         check_swiglu(x[keep], xs[keep], g, gs, u, us, q[keep], s[keep])
 
 
+@pytest.mark.parametrize("M,N", [(1, 144), (5, 2064), (33, 272), (130, 144), (300, 2064), (700, 272)])
+def test_linear_swiglu_writes_only_its_own(M, N):
+    """Padded outputs with a guard row: what lies between and behind the rows stays as it was, in both forms
+    and with a last block of 16 outputs."""
+    K = 272
+    x, xs = F.make(M, K, 1, seed=1, device="cuda")
+    g, gs = F.make(N, K, 128, seed=2, device="cuda")
+    u, us = F.make(N, K, 128, seed=3, device="cuda")
+    q, s = fp8.linear_swiglu(x, xs, g, gs, u, us)
+    nb = -(-N // 128)
+    qb = torch.full((M + 1, N + 32), 0x55, dtype=torch.uint8, device="cuda")
+    sb = torch.full((M + 1, nb + 3), 0x55, dtype=torch.uint8, device="cuda")
+    L.check(L.load().ixb_fp8_linear_swiglu(x.data_ptr(), K, xs.data_ptr(), xs.stride(0), g.data_ptr(), K, gs.data_ptr(), gs.stride(0),
+                                           u.data_ptr(), K, us.data_ptr(), us.stride(0), qb.data_ptr(), N + 32, sb.data_ptr(), nb + 3,
+                                           M, N, K, None))
+    settle()
+    assert torch.equal(qb[:M, :N], q.view(torch.uint8)) and torch.equal(sb[:M, :nb], s.view(torch.uint8))
+    assert (qb[:, N:] == 0x55).all() and (qb[M] == 0x55).all() and (sb[:, nb:] == 0x55).all() and (sb[M] == 0x55).all()
+
+
+@pytest.mark.parametrize("M", [1, 40, 500])
+def test_gate_and_up_as_views_of_one_weight(M):
+    K, N = 528, 400
+    x, xs = F.make(M, K, 1, seed=1, device="cuda")
+    g, gs = F.make(N, K, 128, seed=2, device="cuda")
+    u, us = F.make(N, K, 128, seed=3, device="cuda")
+    both = torch.cat([g.view(torch.uint8), u.view(torch.uint8)]).view(fp8.E4M3)
+    q, s = fp8.linear_swiglu(x, xs, both[:N], gs, both[N:], us)
+    q1, s1 = fp8.linear_swiglu(x, xs, g, gs, u, us)
+    settle()
+    assert same_bits(q, q1) and same_bits(s, s1)
+
+
 # ---------------------------------------------------------------- together
 def layer(tokens, hidden, inner, seed):
     """Weights and inputs of norm -> gate/up -> down."""
@@ -414,6 +465,38 @@ def test_a_decoder_mlp_on_other_streams_and_in_a_graph(tokens):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     settle()
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Nothing that a first call sets up (kernel attributes, the tensor-map encoder) is closed to a capture."""
+    code = """
+import torch
+from ignite_xdna_b200 import fp8
+x = torch.randn(5, 512, device="cuda").bfloat16()
+many = torch.randn(400, 512, device="cuda").bfloat16()
+w = torch.randn(256, 512, device="cuda").bfloat16()
+nw = torch.ones(512, device="cuda").bfloat16()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+def step(x):
+    wq, ws = fp8.quantize(w, block_rows=128)
+    q, s, _ = fp8.rmsnorm_quant(x, nw)
+    q2, s2 = fp8.linear_swiglu(q, s, wq, ws, wq, ws)
+    return fp8.linear(q, s, wq, ws), q2, s2
+with torch.cuda.graph(g):
+    outs = step(x) + step(many)
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(outs, step(x) + step(many)):
+    assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+print("captured")
+"""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr
 
 
 def test_the_int8_norm_feeds_the_w4a8_product():
@@ -498,6 +581,31 @@ def test_refusals():
     with pytest.raises(L.IxbError):
         fp8.rmsnorm_quant(b, nw, position=99)
     settle()
+
+
+def test_two_devices_in_one_process():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU is visible")
+    for dev in ("cuda:0", "cuda:1"):  # the current device stays 0
+        x, xs = F.make(40, 512, 1, 0, device=dev)
+        w, ws = F.make(256, 512, 128, 1, device=dev)
+        out = fp8.linear(x, xs, w, ws)
+        torch.cuda.synchronize(dev)
+        assert out.device == x.device
+        check_product(x, xs, w, ws, out)
+    with pytest.raises(ValueError, match="cuda"):
+        fp8.linear(x, xs, w.to("cuda:0"), ws)
+
+
+def test_what_requires_grad_is_refused_and_no_grad_allows_it():
+    x = randn(3, 256, seed=1, dtype=torch.bfloat16)
+    w = torch.nn.Parameter(torch.ones(256, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError, match="grad"):
+        fp8.rmsnorm_quant(x, w)
+    with torch.no_grad():
+        q, s, _ = fp8.rmsnorm_quant(x, w)
+    settle()
+    assert not q.requires_grad
 
 
 def test_an_inference_mode_tensor_and_a_single_row_view():
