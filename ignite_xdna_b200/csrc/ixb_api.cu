@@ -1055,10 +1055,11 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
     p.kb_split = kbs;
     p.nacc = nacc;
   };
-  // The estimates are microseconds, fitted to 900 timed plans of 66 shapes (1 to 8192 tokens), the large ones
-  // under the power cap: the plan they choose was 1 % slower than the fastest on average.
+  // The estimates are microseconds, fitted to 886 timed plans of 57 shapes (1 to 8192 tokens; large ones in
+  // bursts and under the power cap): the plan they choose was 0.6 % slower than the fastest on
+  // average, 12 % at the worst.
   // Few tokens: a CTA per tile and part of K, two of them on an SM at a time, which hide one another's
-  // latency (a K-block takes a CTA 0.38 us alone) until the operands' arrival or the MMAs bound both.
+  // latency (a K-block takes a CTA 0.37 us alone) until the operands' arrival or the MMAs bound both.
   {
     const int mt = mode == FP8_SWIGLU ? 2 : 1;
     for (int bn = 16; bn <= std::min(kFp8FewTokens, round_up(M, 16)); bn += 16) {
@@ -1070,10 +1071,10 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
         if (split > 1 && ((split - 1) * kbs >= p.kblocks || tiles * split > 9LL * sms / 5)) break;
         const long long per_sm = (tiles * split + sms - 1) / sms;
         auto round = [&](int ctas) {
-          return kbs * std::max(0.384, ctas * std::max(mt * bn * 0.00207, stage * 7.8e-6)) + ctas * mt * bn * 0.025;
+          return kbs * std::max(0.371, ctas * std::max(mt * bn * 0.00259, stage * 7.54e-6)) + ctas * mt * bn * 0.03;
         };
         const long long pairs = (per_sm - 1) / 2;  // whole rounds of two before the last
-        take(2.4 + pairs * round(2) + round((int)(per_sm - 2 * pairs)) + (split > 1 ? 0.13 * split : 0.0), 1, mt, bn, split, kbs, 1);
+        take(1.69 + pairs * round(2) + round((int)(per_sm - 2 * pairs)) + (split > 1 ? 0.143 * split : 0.0), 1, mt, bn, split, kbs, 1);
       }
     }
   }
@@ -1082,13 +1083,16 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
     if ((mode == FP8_SWIGLU && mt == 2) || sms < 2) continue;
     const int rows = mode == FP8_SWIGLU ? 1 : 2 * mt;  // weight blocks per tile (of each product)
     for (int bn = 32; bn <= std::min(256, round_up(M, 32)); bn += 32) {
-      const int sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
-      if (mt * bn + sf_cols > 512) break;
+      const int cols = mt * bn, sf_cols = 2 * 4 * (mt + (bn + 127) / 128);
+      if (cols + sf_cols > 512) break;
       const long long tiles = (long long)((nblk + rows - 1) / rows) * ((M + bn - 1) / bn);
       const long long waves = (tiles + sms / 2 - 1) / (sms / 2);
-      const bool two = waves > 1 && 2 * mt * bn + sf_cols <= 512;
-      const double tile = p.kblocks * std::max(mt * bn * 0.001106 + 0.0874, 0.308) + 0.824, epi = mt * bn * 0.01;
-      take(2.36 + (two ? waves * std::max(tile, epi) + epi : waves * (tile + epi)), 2, mt, bn, 1, p.kblocks, two ? 2 : 1);
+      const bool two = waves > 1 && 2 * cols + sf_cols <= 512;
+      const double kb = mode == FP8_SWIGLU ? std::max(cols * 0.000647 + 0.165, 0.228)
+                        : mt == 1          ? std::max(cols * 0.00113 + 0.0724, 0.169)
+                                           : std::max(cols * 0.00118 + 0.0875, 0.334);
+      const double tile = p.kblocks * kb + 1.16, epi = cols * (mode == FP8_SWIGLU ? 0.0206 : 0.00751);
+      take(2.87 + (two ? waves * std::max(tile, epi) + epi : waves * (tile + epi)), 2, mt, bn, 1, p.kblocks, two ? 2 : 1);
     }
   }
   const int mt = L.mt, cg = L.cg;
@@ -1105,7 +1109,8 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   const int groups_n = std::max(1, (int)ceil(p.n_tiles / std::max(1.0, square)));
   p.n_group = (p.n_tiles + groups_n - 1) / groups_n;
   L.grid = (int)(cg == 1 ? tiles * p.split : 2 * std::min<long long>(tiles, sms / 2));
-  p.stage_bytes = mt * kGemmABlock + p.bn * 128 / cg;
+  const int ks = fp8_stage_blocks(mode, mt, cg);
+  p.stage_bytes = ks * (mt * kGemmABlock + p.bn * 128 / cg);
   const int groups = (p.bn + 127) / 128;
   // the persistent form gathers the next tile's scales beside this one's; a CTA with one tile needs what its K has
   const int images = cg == 1 ? std::min(kSfSlots, (p.kb_split + kSfSpan - 1) / kSfSpan) : kSfSlots;
@@ -1115,7 +1120,7 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   // the few-token form leaves room for a second CTA (1 KB of each SM's 228 is the system's, per CTA)
   const int limit = cg == 1 ? kSmemLimit / 2 - 1024 : kSmemLimit;
   const int red = cg == 1 ? (mt * p.bn * 512 + p.stage_bytes - 1) / p.stage_bytes : 1;
-  p.stages = std::max(std::min(std::min(kFp8MaxStages, (limit - fixed) / p.stage_bytes), p.kb_split), red);
+  p.stages = std::max(std::min(std::min(kFp8MaxStages, (limit - fixed) / p.stage_bytes), (p.kb_split + ks - 1) / ks), red);
   p.sf_off = p.stages * p.stage_bytes;
   p.stg_off = p.sf_off + sf;
   p.bar_off = p.stg_off + stg;

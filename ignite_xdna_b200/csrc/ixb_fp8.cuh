@@ -508,6 +508,13 @@ struct Fp8Params {
   long long ldq, ldqs;
 };
 
+// K-blocks per stage. A turn of the MMA warp's loop (look at a barrier, elect, four MMAs, commit) takes ~440
+// cycles, the MMAs of a pair's K-block with 128 tokens 256: two K-blocks to a turn where the pair's
+// stages leave room (512 x 4096 x 11008 26.8 -> 24.5 us). The swiglu pairs hold their exchange too, and
+// three stages of two measured slower than six of one (2048 x 11008 x 4096 146 us instead of 142).
+__host__ __device__ constexpr int fp8_stage_blocks(int mode, int mt, int cg) {
+  return cg == 2 && mt == 1 && mode == FP8_LINEAR ? 2 : 1;
+}
 // Instruction descriptor of tcgen05.mma kind::mxf8f6f4: e4m3 x e4m3 -> f32, both K-major, e8m0 scales.
 __host__ __device__ constexpr uint32_t umma_idesc_mxf8(int m, int n) {
   return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
@@ -652,12 +659,39 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
 __device__ __forceinline__ void scale_copy(void* dst, const uint8_t* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
-// The same word byte by byte (1..4 of them), in a register. No branch: the loads of many rows overlap.
-__device__ __forceinline__ uint32_t scale_bytes(const uint8_t* src, int bytes) {
-  uint32_t w = __ldg(src);
+// The five aligned words that hold the 16 bytes from `src`; what lies at or past `end` (the matrix's) reads as 0.
+// Predicated, without branches, so that the loads of many rows overlap. Returns whether `end` cuts one of
+// the words: its bytes are missing.
+// ORDERED: kept apart from the memory accesses around it, which holds fewer registers.
+template <bool ORDERED>
+__device__ __forceinline__ bool scale_words5(const uint8_t* src, const uint8_t* end, uint32_t (&w)[5]) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(src) & ~uintptr_t(3), e = reinterpret_cast<uintptr_t>(end);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) w |= (uint32_t)__ldg(src + min(i, bytes - 1)) << (8 * i);
-  return w;  // bytes past the last block repeat it; no MMA reads them
+  for (int i = 0; i < 5; ++i) {
+    const uint32_t in = a + 4 * i + 4 <= e;
+#define IXB_LOAD_IF                    \
+  "{\n\t.reg .pred p;\n\t"            \
+  "setp.ne.b32 p, %2, 0;\n\t"          \
+  "mov.b32 %0, 0;\n\t"                 \
+  "@p ld.global.nc.b32 %0, [%1];\n\t}"
+    if constexpr (ORDERED) asm volatile(IXB_LOAD_IF : "=r"(w[i]) : "l"(a + 4 * i), "r"(in) : "memory");
+    else asm(IXB_LOAD_IF : "=r"(w[i]) : "l"(a + 4 * i), "r"(in));
+#undef IXB_LOAD_IF
+  }
+  const uintptr_t t = e & ~uintptr_t(3);
+  return t != e && t >= a && t < a + 20;
+}
+__device__ __forceinline__ void scale_last_bytes(const uint8_t* src, const uint8_t* end, uint32_t (&w)[5]) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(src) & ~uintptr_t(3), e = reinterpret_cast<uintptr_t>(end);
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (a + 4 * i + j < e && a + 4 * i + 4 > e) w[i] |= (uint32_t)*reinterpret_cast<const uint8_t*>(a + 4 * i + j) << (8 * j);
+}
+// Where row i of a lane goes in four K-blocks' images: weight blocks first, then x's groups of 128 rows.
+__device__ __forceinline__ int scale_place(int mt, int i) {
+  return i < mt ? i * kSfAtom : mt * kSfAtom + (i - mt) / 4 * kSfAtom + (i - mt) % 4 * 4;
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
   float4 v;
@@ -818,6 +852,8 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   constexpr int kXRows = CG == 1 ? 4 : 8;  // x rows per lane of a scale image: bn is at most 128, or 256
   const int sfb_groups = CG == 1 ? 1 : (p.bn + 127) / 128;
   const int sf_quad = (MT + sfb_groups) * kSfAtom;  // four K-blocks' images
+  constexpr int KS = fp8_stage_blocks(MODE, MT, CG);
+  const int block_bytes = p.stage_bytes / KS;
 
   grid_dep_launch();
   if (warp == MW) tmem_alloc_cg<CG>(tmem_slot, p.tmem_cols);
@@ -861,24 +897,29 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
     for (int t = tile0; ok && t < tiles; t += tstep) {
       int mt, nt;
       tile_at(p, t, mt, nt);
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += KS) {
         if (!warp_all(mbar_poll(&empty[s], ph ^ 1))) {
           ok = false;
           break;
         }
         uint8_t* st = smem + s * p.stage_bytes;
+        const int n = min(KS, kb1 - kb);
         if (elect_one()) {
-          if (pair == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * p.stage_bytes));
+          if (pair == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * n * block_bytes));
           const uint32_t lead = CG == 2 ? cluster_addr(&full[s], 0) : 0;
 #pragma unroll
-          for (int b = 0; b < MT; ++b) {
-            const CUtensorMap* tw = &p.tw[weight_source<MODE, CG>(pair, b)];
-            const int row = weight_block<MODE, MT, CG>(nt, pair, b) * 128;
-            if (CG == 2) tma_load_2d_pair(st + b * kGemmABlock, tw, kb * 128, row, lead);
-            else tma_load_2d(st + b * kGemmABlock, tw, kb * 128, row, &full[s]);
+          for (int k = 0; k < KS; ++k, st += block_bytes) {
+            if (k >= n) break;
+#pragma unroll
+            for (int b = 0; b < MT; ++b) {
+              const CUtensorMap* tw = &p.tw[weight_source<MODE, CG>(pair, b)];
+              const int row = weight_block<MODE, MT, CG>(nt, pair, b) * 128;
+              if (CG == 2) tma_load_2d_pair(st + b * kGemmABlock, tw, (kb + k) * 128, row, lead);
+              else tma_load_2d(st + b * kGemmABlock, tw, (kb + k) * 128, row, &full[s]);
+            }
+            if (CG == 2) tma_load_2d_pair(st + MT * kGemmABlock, &p.tx, (kb + k) * 128, mt * p.bn + pair * (p.bn / 2), lead);
+            else tma_load_2d(st + MT * kGemmABlock, &p.tx, (kb + k) * 128, mt * p.bn, &full[s]);
           }
-          if (CG == 2) tma_load_2d_pair(st + MT * kGemmABlock, &p.tx, kb * 128, mt * p.bn + pair * (p.bn / 2), lead);
-          else tma_load_2d(st + MT * kGemmABlock, &p.tx, kb * 128, mt * p.bn, &full[s]);
         }
         if (++s == S) {
           s = 0;
@@ -889,8 +930,9 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   } else if (warp == SW) {
     // ------------------------------------------------------------ scale gatherer
     // Words go straight from global to shared memory (cp.async, 4 bytes each, short or absent ones
-    // filled with zeros). Rows whose words are not 4-byte aligned go through registers, a byte at a
-    // time, all of a quad's loads in flight together. An image spans 16 K-blocks because handing one
+    // filled with zeros). Rows whose words are not 4-byte aligned (K / 128 no multiple of 4) go through
+    // registers, five aligned words for 16 K-blocks of a row: a load touches 32 rows, so it is the number
+    // of loads that counts, and byte by byte they held 512 x 4096 x 11008 at 27 us. An image spans 16 K-blocks because handing one
     // over (copies in flight, the proxy fence, the arrival at the other CTA) takes 2,000 cycles, more
     // than four K-blocks' MMAs.
     int s = 0;
@@ -899,21 +941,16 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
     for (int t = tile0; ok && t < tiles; t += tstep) {
       int mt, nt;
       tile_at(p, t, mt, nt);
-      const uint8_t* row[MT + kXRows];  // this lane's rows: the weight blocks', then x's
-      bool in[MT + kXRows];
+      // This lane's rows: the weight blocks', then x's. A row past the matrix or the tile takes the last
+      // one's scales: its operand is zero or no part of the MMA, and its output is not stored.
+      const uint8_t* row[MT + kXRows];
 #pragma unroll
       for (int b = 0; b < MT; ++b) {
         const int src = weight_source<MODE, CG>(pair, b);
-        const long long r = weight_block<MODE, MT, CG>(nt, pair, b);
-        in[b] = r * 128 < p.N;
-        row[b] = p.ws[src] + (in[b] ? r : 0) * p.ldws[src];
+        row[b] = p.ws[src] + min(weight_block<MODE, MT, CG>(nt, pair, b), (p.N - 1) / 128) * p.ldws[src];
       }
 #pragma unroll
-      for (int j = 0; j < kXRows; ++j) {
-        const long long m = (long long)mt * p.bn + j * 32 + lane;
-        in[MT + j] = j * 32 + lane < p.bn && m < p.M;
-        row[MT + j] = p.xs + (in[MT + j] ? m : 0) * p.ldxs;
-      }
+      for (int j = 0; j < kXRows; ++j) row[MT + j] = p.xs + min(mt * p.bn + j * 32 + lane, p.M - 1) * p.ldxs;
       for (int kb = kb0; kb < kb1; kb += kSfSpan) {
         if (!warp_all(mbar_poll(&sf_empty[s], ph ^ 1))) {
           ok = false;
@@ -921,31 +958,53 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
         }
         uint8_t* im = smem + p.sf_off + s * (4 * sf_quad) + lane * 16;
         const int end = min(kb1, kb + kSfSpan);
-        for (int kq = kb; kq < end; kq += 4, im += sf_quad) {
-          const int left = min(4, p.kblocks - kq);
-          if (p.sf_words) {
+        if (p.sf_words) {
+          for (int kq = kb; kq < end; kq += 4, im += sf_quad) {
+            const int left = min(4, p.kblocks - kq);
 #pragma unroll
             for (int i = 0; i < MT + kXRows; ++i) {
-              if (i >= MT + 4 && sfb_groups == 1) continue;
+              if (CG == 1 ? i >= MT && (i - MT) * 32 >= p.bn : i >= MT + 4 && sfb_groups == 1) break;
 #pragma unroll
               for (int j = 0; j < (i < MT ? 4 : 1); ++j)
-                scale_copy(im + (i < MT ? i * kSfAtom + 4 * j : MT * kSfAtom + (i - MT) / 4 * kSfAtom + (i - MT) % 4 * 4), row[i] + kq,
-                           in[i] ? left : 0);
+                scale_copy(im + scale_place(MT, i) + (i < MT ? 4 * j : 0), row[i] + kq, left);
+            }
+          }
+        } else {
+          auto stop = [&](int i) {  // the end of the matrix that row i is of
+            const int src = weight_source<MODE, CG>(pair, i);
+            return (i < MT ? p.ws[src] + (p.N - 1) / 128 * p.ldws[src] : p.xs + (p.M - 1) * p.ldxs) + p.kblocks;
+          };
+          auto place = [&](int i, const uint32_t (&w)[5]) {
+            const uint32_t sh = 8 * (uint32_t)(reinterpret_cast<uintptr_t>(row[i] + kb) & 3);
+#pragma unroll
+            for (int q = 0; q < kSfSpan / 4; ++q) {
+              const uint32_t v = __funnelshift_r(w[q], w[q + 1], sh);
+              uint8_t* at = im + q * sf_quad + scale_place(MT, i);
+              if (i < MT) *reinterpret_cast<uint4*>(at) = make_uint4(v, v, v, v);
+              else *reinterpret_cast<uint32_t*>(at) = v;
+            }
+          };
+          if constexpr (CG == 1) {  // few rows, and few registers: one row after the other
+#pragma unroll
+            for (int i = 0; i < MT + kXRows; ++i) {
+              if (i >= MT && (i - MT) * 32 >= p.bn) break;
+              uint32_t w[5];
+              const bool cut = scale_words5<true>(row[i] + kb, stop(i), w);
+              if (__any_sync(0xffffffffu, cut)) scale_last_bytes(row[i] + kb, stop(i), w);
+              place(i, w);
             }
           } else {
-            uint32_t w[MT + kXRows];
+            uint32_t w[MT + kXRows][5];
+            bool cut = false;
 #pragma unroll
-            for (int i = 0; i < MT + kXRows; ++i) w[i] = scale_bytes(row[i] + kq, left);
+            for (int i = 0; i < MT + kXRows; ++i) cut |= scale_words5<false>(row[i] + kb, stop(i), w[i]);
+            if (__any_sync(0xffffffffu, cut)) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-              *reinterpret_cast<uint4*>(im + i * kSfAtom) = in[i] ? make_uint4(w[i], w[i], w[i], w[i]) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int g = 0; g < kXRows / 4; ++g) {
-              const int i = MT + 4 * g;
-              if (g < sfb_groups)
-                *reinterpret_cast<uint4*>(im + (MT + g) * kSfAtom) =
-                    make_uint4(in[i] ? w[i] : 0, in[i + 1] ? w[i + 1] : 0, in[i + 2] ? w[i + 2] : 0, in[i + 3] ? w[i + 3] : 0);
+              for (int i = 0; i < MT + kXRows; ++i) scale_last_bytes(row[i] + kb, stop(i), w[i]);
             }
+#pragma unroll
+            for (int i = 0; i < MT + kXRows; ++i)
+              if (i < MT + 4 || sfb_groups == 2) place(i, w[i]);
           }
         }
         cp_async_commit();
@@ -976,6 +1035,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       const uint64_t ad0 = umma_desc_sw128(smem_u32(smem));
       uint64_t ad = ad0;
       bool ready = false;
+      constexpr uint32_t kNextScale = (1u << 29) | (1u << 4);  // the next byte of both scale words
       for (int t = tile0; ok && t < tiles; t += tstep) {
         if (!warp_all(mbar_wait_cg<CG>(&acc_empty[acc], aph ^ 1))) break;
         tc_fence_after();
@@ -996,7 +1056,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             sfbuf ^= 1;
             uint32_t idesc = p.idesc;
             const int n = min(4, end - kq);
-            for (int i = 0; i < n; ++i) {
+            for (int i = 0; i < n; i += KS) {
               if (!ready && !warp_all(mbar_poll(&full[s], ph))) {
                 ok = false;
                 break;
@@ -1005,17 +1065,21 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
               const int s1 = s + 1 == S ? 0 : s + 1;
               const bool next = mbar_test(&full[s1], ph ^ (s1 == 0 ? 1u : 0u));  // looked at while the MMAs are issued
               if (elect_one()) {
-                const uint64_t bd = ad + MT * (kGemmABlock >> 4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int k = 0; k < KS; ++k) {
+                  if (i + k >= n) break;
+                  const uint64_t a = ad + k * (uint32_t)(block_bytes >> 4), bd = a + MT * (kGemmABlock >> 4);
 #pragma unroll
-                  for (int b = 0; b < MT; ++b)
-                    umma_mxf8<CG>(d0 + b * p.bn, ad + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, idesc, sf + 4 * b, sf + 4 * MT,
-                                  j ? 1u : accumulate);
+                  for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int b = 0; b < MT; ++b)
+                      umma_mxf8<CG>(d0 + b * p.bn, a + b * (kGemmABlock >> 4) + 2 * j, bd + 2 * j, idesc + k * kNextScale, sf + 4 * b,
+                                    sf + 4 * MT, j || k ? 1u : accumulate);
+                }
                 umma_commit_cg<CG>(&empty[s]);
               }
               ready = warp_all(next);
-              idesc += (1u << 29) | (1u << 4);  // the next byte of both scale words
+              idesc += KS * kNextScale;
               accumulate = 1;
               issued = true;
               ad += dstep;
