@@ -9,8 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_strided.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -139,12 +138,12 @@ Operand operand(const at::Tensor& first, PyObject* qo, PyObject* so, const char*
 }
 
 at::Tensor matrix(int64_t rows, int64_t cols, const at::Tensor& like, at::ScalarType type) {
-  return at::empty({rows, cols}, like.options().dtype(type).requires_grad(false));
+  return at::Tensor(at::detail::empty_cuda({rows, cols}, type, like.device(), std::nullopt));
 }
 // An empty scale matrix whose rows start on 4 bytes, which the products read a word at a time.
 at::Tensor scales(int64_t rows, int64_t cols, const at::Tensor& like) {
   const int64_t n = blocks(cols);
-  return at::empty_strided({rows, n}, {(n + 3) / 4 * 4, 1}, like.options().dtype(at::kFloat8_e8m0fnu).requires_grad(false));
+  return at::Tensor(at::detail::empty_strided_cuda({rows, n}, {(n + 3) / 4 * 4, 1}, at::kFloat8_e8m0fnu, like.device()));
 }
 uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.mutable_data_ptr()); }
 
