@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -269,6 +270,13 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, x_scal
       if (ldo < N) ldo = N;
       same_shape(out, M, N, "out");
       same_device(x, out, "out");
+      for (int i = 0; i < 4; ++i) {
+        const auto overlap = at::get_overlap_status(THPVariable_Unpack(a[i]), out);
+        if (overlap == at::MemOverlapStatus::Full || overlap == at::MemOverlapStatus::Partial)
+          raise(PyExc_ValueError, "out shares memory with an input");
+      }
+      // what autograd has saved of it is no longer what it saved
+      if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     }
     check(fp8_linear(ox.q, ox.ld, ox.s, ox.lds, ow.q, ow.ld, ow.s, ow.lds, out.mutable_data_ptr(), type_of(out, "out"), ldo, (int)M,
                      (int)N, (int)K, on.stream));

@@ -319,8 +319,9 @@ int ixb_rmsnorm_quant(const void* x, int64_t ldx, const void* residual, int64_t 
                       uint8_t* scale, int64_t lds, void* stream);
 /* out [M][N] of out_type = x . w^T: x [M][K] with its scales, w [N][K] with its blocks'. Sums in fp32 on the
  * tensor cores (tcgen05 kind::mxf8f6f4, which multiplies the scales in), one rounding at the end. The
- * order of a sum depends on M, N and K alone. N in [1, 2^24], K at most 65536 (a sum's relative error
- * grows with K: 1e-7 at 4096, 3e-6 at 65536, as fp32 products of normal values). */
+ * order of a sum depends on M, N, K and the device's SMs alone. N in [1, 2^24], K at most 65536 (the tensor
+ * cores cut where they align, so a sum's relative error grows with K and with the spread of its terms:
+ * 1e-7 at 4096 and 3e-6 at 65536 for normal values, 4e-7 at 4096 where a few columns are far larger). */
 int ixb_fp8_linear(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldxs, const uint8_t* w, int64_t ldw,
                    const uint8_t* w_scale, int64_t ldws, void* out, int out_type, int64_t ldo, int M, int N, int K,
                    void* stream);

@@ -605,3 +605,38 @@ def test_an_inference_mode_tensor_and_a_single_row_view():
         one = fp8.linear(x[2:3], xs[2:3], w, ws)
         settle()
         assert torch.equal(one, every[2:3])
+
+
+def test_out_that_shares_memory_with_an_input_is_refused():
+    x, xs = F.make(64, 512, 1, 0, device="cuda")
+    w, ws = F.make(256, 512, 128, 1, device="cuda")
+    buf = torch.zeros(256 * 512, dtype=torch.uint8, device="cuda")
+    out = buf.view(torch.bfloat16)[-64 * 256:].view(64, 256)
+    shared = buf.view(torch.float8_e4m3fn).view(256, 512)
+    shared.copy_(w)
+    before = buf.clone()
+    with pytest.raises(ValueError, match="shares memory"):
+        fp8.linear(x, xs, shared, ws, out=out)
+    settle()
+    assert torch.equal(buf, before)
+    head = buf.view(torch.float8_e4m3fn)[:128 * 512].view(128, 512)  # beside it in one buffer is no overlap
+    tail = buf.view(torch.bfloat16)[-64 * 128:].view(64, 128)
+    fp8.linear(x, xs, head, ws[:1], out=tail)
+    settle()
+    assert torch.equal(tail, fp8.linear(x, xs, w[:128], ws[:1]))
+
+
+def test_writing_out_is_seen_by_autograd():
+    """A tensor that a graph has saved is written: the backward pass raises and does not use the new values."""
+    x, xs = F.make(8, 256, 1, 0, device="cuda")
+    w, ws = F.make(128, 256, 128, 1, device="cuda")
+    out = torch.ones(8, 128, dtype=torch.float32, device="cuda")
+    leaf = torch.ones(8, 128, device="cuda", requires_grad=True)
+    y = (leaf * out).sum()
+    fp8.linear(x, xs, w, ws, out=out)
+    settle()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # tensors without a version
+        fp8.linear(x, xs, w, ws, out=torch.empty(8, 128, device="cuda"))
+    settle()
