@@ -927,6 +927,13 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
         }
       }
     }
+    // The releases of the last stages, which the pair's leader sends to both CTAs, have arrived before this CTA
+    // leaves: a signal still on its way would reach the shared memory of whoever has it next.
+    for (int i = 0; i < S && warp_all(mbar_poll(&empty[s], ph ^ 1)); ++i)
+      if (++s == S) {
+        s = 0;
+        ph ^= 1;
+      }
   } else if (warp == SW) {
     // ------------------------------------------------------------ scale gatherer
     // Words go straight from global to shared memory (cp.async, 4 bytes each, short or absent ones
@@ -1021,6 +1028,11 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
         }
       }
     }
+    for (int i = 0; i < kSfSlots && warp_all(mbar_poll(&sf_empty[s], ph ^ 1)); ++i)  // as the producer
+      if (++s == kSfSlots) {
+        s = 0;
+        ph ^= 1;
+      }
   } else if (warp == MW) {
     // ------------------------------------------------------------ MMA issuer
     // The tensor core's queue holds little more than the MMA it works on, so what this warp does between
@@ -1103,10 +1115,18 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
           aph ^= 1;
         }
       }
+      if (CG == 2)  // the other CTA's last releases of an accumulator are here
+        for (int i = 0; i < p.nacc && warp_all(mbar_wait_cg<CG>(&acc_empty[acc], aph ^ 1)); ++i)
+          if (++acc == p.nacc) {
+            acc = 0;
+            aph ^= 1;
+          }
       if (issued) {
         if (elect_one()) umma_commit_cg<CG>(done);  // every MMA this CTA issued has finished before TMEM is released
         mbar_poll(done, 0);
       }
+    } else {
+      mbar_poll(done, 0);  // the leader's commit arrives in both CTAs: the last signal that this one gets
     }
   } else if constexpr (CG == 2) {
     // ------------------------------------------------------------ epilogue
@@ -1271,8 +1291,8 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   }
   tc_fence_before();
   __syncthreads();
-  // no CTA leaves while another reads its shared memory (parts of a tile), or while the pair's MMAs and
-  // signals reach it
+  // no CTA leaves while another reads its shared memory (parts of a tile). What else reaches a CTA of a pair
+  // from the other one has been waited for: the barrier says nothing about signals and copies under way.
   cluster_sync();
   tc_fence_after();
   if (warp == MW) tmem_dealloc_cg<CG>(tmem, p.tmem_cols);
