@@ -1063,6 +1063,7 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   {
     const int mt = mode == FP8_SWIGLU ? 2 : 1;
     for (int bn = 16; bn <= std::min(kFp8FewTokens, round_up(M, 16)); bn += 16) {
+      if (mt * bn + 2 * 4 * (mt + 1) > kFp8FewTmem) break;
       const long long tiles = (long long)nblk * ((M + bn - 1) / bn);
       const int stage = mt * kGemmABlock + bn * 128;
       for (int split = 1; split <= kFp8MaxSplit; ++split) {
@@ -1124,13 +1125,13 @@ int plan_fp8(Fp8Launch& L, int M, int N, int K, int mode, std::string& err) {
   p.sf_off = p.stages * p.stage_bytes;
   p.stg_off = p.sf_off + sf;
   p.bar_off = p.stg_off + stg;
-  L.smem = fixed + p.sf_off;
+  L.smem = cg == 1 ? std::max(fixed + p.sf_off, kFp8FewShared) : kSmemLimit;
   p.acc_cols = mt * p.bn;
   const int need = p.nacc * p.acc_cols + 2 * 4 * (mt + groups);
   p.tmem_cols = 32;
   while (p.tmem_cols < need) p.tmem_cols *= 2;
   p.idesc = umma_idesc_mxf8(128 * cg, p.bn);
-  if (L.smem > kSmemLimit || p.tmem_cols > 512 || p.stages > kFp8MaxStages) {
+  if (fixed + p.sf_off > L.smem || L.smem > kSmemLimit || p.tmem_cols > (cg == 1 ? kFp8FewTmem : 512) || p.stages > kFp8MaxStages) {
     err = "no tile fits";
     return -1;
   }

@@ -486,6 +486,14 @@ constexpr int kFp8SwapBytes = kFp8Epi * 2 * kFp8WarpSwap;
 constexpr int kFp8TopBytes = 2 * 2 * kFp8Chunk * 4 * 4;
 constexpr int kFp8SwapBar = 384;
 constexpr int kFp8BarBytes = 512;
+// A TMEM allocation waits, without a limit, for the columns that other CTAs of the SM hold, and the CTAs of a
+// cluster wait for one another. Two clusters on two streams must not each hold columns on one SM that the other
+// needs on another: so a CTA of the few-token form takes at most half of TMEM, and at least the shared memory
+// that lets two CTAs onto an SM and no third; a CTA of a pair takes all shared memory and is alone.
+constexpr int kFp8FewTmem = 256;
+constexpr int kSmShared = 228 * 1024;  // an SM's shared memory; the system takes 1 KB of it per CTA
+constexpr int kFp8FewShared = kSmShared / 3 - 1024 + 128;
+static_assert(3 * (kFp8FewShared + 1024) > kSmShared, "no third CTA");
 enum : int { FP8_LINEAR = 0, FP8_SWIGLU = 1 };
 
 struct Fp8Params {
@@ -855,7 +863,6 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   constexpr int KS = fp8_stage_blocks(MODE, MT, CG);
   const int block_bytes = p.stage_bytes / KS;
 
-  grid_dep_launch();
   if (warp == MW) tmem_alloc_cg<CG>(tmem_slot, p.tmem_cols);
   if (tid == PW * 32) {
     for (int s = 0; s < S; ++s) {
@@ -883,6 +890,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   if (CG == 2) cluster_sync();  // both CTAs' barriers exist before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_dep_launch();  // not before this CTA has its TMEM: the next kernel's CTAs would hold theirs until this grid ends
   bool part_ok = true;
   grid_dep_wait();  // x, the scales, and whatever still reads the outputs, from here on
 

@@ -1,0 +1,25 @@
+"""The fp8 products' launch plans, without a GPU: what keeps launches on several streams from waiting for one another,
+and that the GPU tests reach every form."""
+import random
+
+import pytest
+
+from test_fp8 import plan
+
+SM_SHARED, SYSTEM = 228 * 1024, 1024  # an SM's shared memory, and what the system takes of it per CTA
+SIZES = [1, 7, 16, 17, 40, 64, 100, 112, 113, 120, 127, 128, 129, 240, 256, 400, 512, 1537, 4096]
+
+
+@pytest.mark.parametrize("swiglu", [0, 1])
+def test_clusters_cannot_wait_for_one_anothers_tmem(swiglu):
+    """An allocation waits for the columns of the SM's other CTAs, and a cluster's CTAs for one another. Few tokens: two CTAs
+    per SM at the most, each with at most half of TMEM. Pairs: alone on their SMs."""
+    r = random.Random(1)
+    depths = [16, 144, 256, 528, 2064, 4096, 11008, 12880] + [16 * r.randint(1, 1024) for _ in range(30)]
+    cases = [(120, 3664, 12880)] + [(M, N, K) for M in SIZES for N in (16, 144, 1024, 3664, 11008) for K in depths]
+    for M, N, K in cases:
+        p = plan(M, N, K, swiglu)
+        if p["cg"] == 1:
+            assert p["tmem"] <= 256 and 3 * (p["smem"] + SYSTEM) > SM_SHARED, (M, N, K, p)
+        else:
+            assert p["tmem"] <= 512 and p["smem"] + SYSTEM == SM_SHARED, (M, N, K, p)
