@@ -639,6 +639,19 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
   set_dev_error(DEV_ERR_WAIT_TIMEOUT);
   return false;
 }
+// A wait for what is on its way whether or not some other wait has given up (copies into this CTA's shared memory,
+// MMAs into its TMEM): with the same limit, but the flag does not end it.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_settle(uint64_t* bar, uint32_t parity, unsigned long long t0 = 0) {  // t0: 0 is now
+  if (mbar_try<CLUSTER>(bar, parity)) return true;
+  if (t0 == 0) t0 = global_ns();
+  while (!mbar_try<CLUSTER>(bar, parity))
+    if (global_ns() - t0 > kWaitLimitNs) {
+      set_dev_error(DEV_ERR_WAIT_TIMEOUT);
+      return false;
+    }
+  return true;
+}
 // The wait's outcome as one value of the warp: a branch on it leaves the code after it uniform.
 __device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xffffffffu, ok); }
 // A bounded wait for arrivals of the other CTA of a pair too.
@@ -936,12 +949,18 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
       }
     }
     // The releases of the last stages, which the pair's leader sends to both CTAs, have arrived before this CTA
-    // leaves: a signal still on its way would reach the shared memory of whoever has it next.
-    for (int i = 0; i < S && warp_all(mbar_poll(&empty[s], ph ^ 1)); ++i)
+    // leaves: a signal still on its way would reach the shared memory of whoever has it next. After a wait
+    // that gave up nothing may read the last stages, and their copies have to land all the same (a pair's count on
+    // the leader's barriers, and its other CTA stays until the leader is done).
+    const unsigned long long t0 = global_ns();
+    for (int i = 0; i < S; ++i) {
+      ok = ok && warp_all(mbar_poll(&empty[s], ph ^ 1));
+      if (!ok && pair == 0) mbar_settle(&full[s], ph ^ 1, t0);
       if (++s == S) {
         s = 0;
         ph ^= 1;
       }
+    }
   } else if (warp == SW) {
     // ------------------------------------------------------------ scale gatherer
     // Words go straight from global to shared memory (cp.async, 4 bytes each, short or absent ones
@@ -1131,10 +1150,10 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
           }
       if (issued) {
         if (elect_one()) umma_commit_cg<CG>(done);  // every MMA this CTA issued has finished before TMEM is released
-        mbar_poll(done, 0);
+        mbar_settle(done, 0);
       }
     } else {
-      mbar_poll(done, 0);  // the leader's commit arrives in both CTAs: the last signal that this one gets
+      mbar_settle(done, 0);  // the leader's commit arrives in both CTAs: the last signal that this one gets
     }
   } else if constexpr (CG == 2) {
     // ------------------------------------------------------------ epilogue
@@ -1216,7 +1235,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
           uint32_t v[kFp8Chunk], u[kFp8Chunk];
           tmem_ld16(base + i * 2 * kFp8Chunk + pair * kFp8Chunk, v);
           if (lane == 0) mbar_arrive_expect_tx(&swap[rbuf], kFp8WarpSwap);
-          ok = mbar_poll<true>(&swap[rbuf], rph) && ok;
+          ok = mbar_settle<true>(&swap[rbuf], rph) && ok;  // the peer sends every run, after a wait that gave up too
 #pragma unroll
           for (int e = 0; e < kFp8Chunk; e += 4) {
             const uint4 w = *reinterpret_cast<const uint4*>(recv + rbuf * kFp8WarpSwap + e * (32 * 4));
