@@ -1142,12 +1142,6 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
           aph ^= 1;
         }
       }
-      if (CG == 2)  // the other CTA's last releases of an accumulator are here
-        for (int i = 0; i < p.nacc && warp_all(mbar_wait_cg<CG>(&acc_empty[acc], aph ^ 1)); ++i)
-          if (++acc == p.nacc) {
-            acc = 0;
-            aph ^= 1;
-          }
       if (issued) {
         if (elect_one()) umma_commit_cg<CG>(done);  // every MMA this CTA issued has finished before TMEM is released
         mbar_settle(done, 0);
@@ -1318,8 +1312,9 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
   }
   tc_fence_before();
   __syncthreads();
-  // no CTA leaves while another reads its shared memory (parts of a tile). What else reaches a CTA of a pair
-  // from the other one has been waited for: the barrier says nothing about signals and copies under way.
+  // No CTA leaves while another reads its shared memory (parts of a tile), or before the arrivals that the other
+  // one's threads made at it (they come before those threads' arrival here). What comes on its own, tcgen05.commit,
+  // copies and st.async, has been waited for: the barrier says nothing about it.
   cluster_sync();
   tc_fence_after();
   if (warp == MW) tmem_dealloc_cg<CG>(tmem, p.tmem_cols);
