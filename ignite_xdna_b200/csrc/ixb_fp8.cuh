@@ -203,13 +203,15 @@ __device__ __forceinline__ uint2 round8(float (&f)[8], float m) {
 }
 
 // ---------------------------------------------------------------- quantise
+// The pointers carry no __restrict__: the kernel before may still be writing x when one of these starts, so its
+// loads must not become loads of read-only data.
 // Rows in blocks of 1 x 128: 16 lanes per block, eight values per lane. Bound by HBM.
 constexpr int kQThreads = 256;
 constexpr int kQUnroll = 4;  // blocks per half-warp, so four 16-byte loads per lane are in flight
 template <typename T>
 __global__ void __launch_bounds__(kQThreads)
-    quantize_rows_kernel(const T* __restrict__ x, long long ldx, int K, FastDiv kb, uint32_t blocks, uint8_t* __restrict__ q,
-                         long long ldq, uint8_t* __restrict__ scale, long long lds) {
+    quantize_rows_kernel(const T* x, long long ldx, int K, FastDiv kb, uint32_t blocks, uint8_t* q, long long ldq, uint8_t* scale,
+                         long long lds) {
   grid_dep_launch();
   grid_dep_wait();
   const int l16 = threadIdx.x & 15;
@@ -247,8 +249,7 @@ __global__ void __launch_bounds__(kQThreads)
 constexpr int kTileThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2)
-    quantize_tiles_kernel(const T* __restrict__ x, long long ldx, int M, int K, uint8_t* __restrict__ q, long long ldq,
-                          uint8_t* __restrict__ scale, long long lds) {
+    quantize_tiles_kernel(const T* x, long long ldx, int M, int K, uint8_t* q, long long ldq, uint8_t* scale, long long lds) {
   constexpr int V = 128 * 128 / 8 / kTileThreads, kStep = kTileThreads / 16;  // rows between a thread's vectors
   grid_dep_launch();
   grid_dep_wait();
@@ -683,21 +684,21 @@ __device__ __forceinline__ void scale_copy(void* dst, const uint8_t* src, uint32
 // The five aligned words that hold the 16 bytes from `src`; what lies at or past `end` (the matrix's) reads as 0.
 // Predicated, without branches, so that the loads of many rows overlap. Returns whether `end` cuts one of
 // the words: its bytes are missing.
-// ORDERED: kept apart from the memory accesses around it, which holds fewer registers.
-template <bool ORDERED>
+// Plain loads in program order: the kernel that writes x's scales may still be running when this one starts, so
+// they are no read-only data, and none may move above the wait for it.
 __device__ __forceinline__ bool scale_words5(const uint8_t* src, const uint8_t* end, uint32_t (&w)[5]) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(src) & ~uintptr_t(3), e = reinterpret_cast<uintptr_t>(end);
 #pragma unroll
   for (int i = 0; i < 5; ++i) {
     const uint32_t in = a + 4 * i + 4 <= e;
-#define IXB_LOAD_IF                    \
-  "{\n\t.reg .pred p;\n\t"            \
-  "setp.ne.b32 p, %2, 0;\n\t"          \
-  "mov.b32 %0, 0;\n\t"                 \
-  "@p ld.global.nc.b32 %0, [%1];\n\t}"
-    if constexpr (ORDERED) asm volatile(IXB_LOAD_IF : "=r"(w[i]) : "l"(a + 4 * i), "r"(in) : "memory");
-    else asm(IXB_LOAD_IF : "=r"(w[i]) : "l"(a + 4 * i), "r"(in));
-#undef IXB_LOAD_IF
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %2, 0;\n\t"
+        "mov.b32 %0, 0;\n\t"
+        "@p ld.global.b32 %0, [%1];\n\t}"
+        : "=r"(w[i])
+        : "l"(a + 4 * i), "r"(in)
+        : "memory");
   }
   const uintptr_t t = e & ~uintptr_t(3);
   return t != e && t >= a && t < a + 20;
@@ -1023,7 +1024,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             for (int i = 0; i < MT + kXRows; ++i) {
               if (i >= MT && (i - MT) * 32 >= p.bn) break;
               uint32_t w[5];
-              const bool cut = scale_words5<true>(row[i] + kb, stop(i), w);
+              const bool cut = scale_words5(row[i] + kb, stop(i), w);
               if (__any_sync(0xffffffffu, cut)) scale_last_bytes(row[i] + kb, stop(i), w);
               place(i, w);
             }
@@ -1031,7 +1032,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
             uint32_t w[MT + kXRows][5];
             bool cut = false;
 #pragma unroll
-            for (int i = 0; i < MT + kXRows; ++i) cut |= scale_words5<false>(row[i] + kb, stop(i), w[i]);
+            for (int i = 0; i < MT + kXRows; ++i) cut |= scale_words5(row[i] + kb, stop(i), w[i]);
             if (__any_sync(0xffffffffu, cut)) {
 #pragma unroll
               for (int i = 0; i < MT + kXRows; ++i) scale_last_bytes(row[i] + kb, stop(i), w[i]);

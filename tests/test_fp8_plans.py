@@ -1,6 +1,8 @@
 """The fp8 products' launch plans, without a GPU: what keeps launches on several streams from waiting for one another,
 and that the GPU tests reach every form."""
 import random
+import re
+from pathlib import Path
 
 import pytest
 
@@ -23,3 +25,19 @@ def test_clusters_cannot_wait_for_one_anothers_tmem(swiglu):
             assert p["tmem"] <= 256 and 3 * (p["smem"] + SYSTEM) > SM_SHARED, (M, N, K, p)
         else:
             assert p["tmem"] <= 512 and p["smem"] + SYSTEM == SM_SHARED, (M, N, K, p)
+
+
+def kernels(name):
+    """The source without comments, and its parts: from one kernel's __global__ to the next."""
+    text = (Path(__file__).resolve().parent.parent / "ignite_xdna_b200" / "csrc" / name).read_text()
+    text = re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
+    return text, text.split("__global__")[1:]
+
+
+def test_fp8_kernels_read_nothing_as_read_only():
+    """Each of them may start while the kernel that writes its inputs runs (programmatic dependent launch), so no load
+    may be one of data that is read-only for the whole kernel: no .nc load, no __ldg, and no const __restrict__ pointer,
+    which lets the compiler make one."""
+    text, parts = kernels("ixb_fp8.cuh")
+    assert all("grid_dep_wait" in k for k in parts) and len(parts) == 4
+    assert not re.search(r"\.nc\b|__ldg|__restrict__", text)
