@@ -9,7 +9,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -111,6 +110,31 @@ void same_shape(const at::Tensor& t, int64_t rows, int64_t cols, const char* nam
 void same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
   if (a.device() != b.device())
     raise(PyExc_ValueError, "%s: on %s, the others on %s", name, b.device().str().c_str(), a.device().str().c_str());
+}
+
+// Whether two matrices with contiguous rows have a byte in common. Exact where their rows are equally far apart
+// (two column ranges of one matrix) or either has one row; elsewhere matrices whose spans meet count as sharing.
+bool shares_memory(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  struct Rows {
+    int64_t begin, width, pitch, rows;  // bytes
+    explicit Rows(const at::Tensor& t) {
+      const int64_t size = (int64_t)t.element_size();
+      begin = (int64_t)reinterpret_cast<intptr_t>(t.const_data_ptr());
+      width = t.size(1) * size;
+      rows = t.size(0);
+      pitch = rows > 1 ? t.stride(0) * size : width;
+    }
+    int64_t end() const { return begin + (rows - 1) * pitch + width; }
+  } x(a), y(b);
+  if (x.begin >= y.end() || y.begin >= x.end()) return false;
+  if (x.rows == 1) x.pitch = y.pitch;
+  if (y.rows == 1) y.pitch = x.pitch;
+  if (x.pitch != y.pitch || x.width > x.pitch || y.width > y.pitch) return true;
+  // the spans meet and both repeat every `pitch` bytes: the rows miss one another if neither's columns, taken
+  // around the pitch, reach into the other's
+  const int64_t d = ((y.begin - x.begin) % x.pitch + x.pitch) % x.pitch;  // from x's columns to y's
+  return d < x.width || d + y.width > x.pitch;
 }
 
 // An e4m3 matrix of K columns with a scale per `rows` rows and 128 columns.
@@ -270,11 +294,8 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x, x_scal
       if (ldo < N) ldo = N;
       same_shape(out, M, N, "out");
       same_device(x, out, "out");
-      for (int i = 0; i < 4; ++i) {
-        const auto overlap = at::get_overlap_status(THPVariable_Unpack(a[i]), out);
-        if (overlap == at::MemOverlapStatus::Full || overlap == at::MemOverlapStatus::Partial)
-          raise(PyExc_ValueError, "out shares memory with an input");
-      }
+      for (int i = 0; i < 4; ++i)
+        if (shares_memory(THPVariable_Unpack(a[i]), out)) raise(PyExc_ValueError, "out shares memory with an input");
       // what autograd has saved of it is no longer what it saved
       if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     }
@@ -303,6 +324,14 @@ PyObject* py_linear_swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {  // x,
   });
 }
 
+PyObject* py_shares_memory(PyObject*, PyObject* const* a, Py_ssize_t n) {  // two matrices with contiguous rows
+  return guarded(n, 2, [&] {
+    const at::Tensor &x = tensor(a[0], "a"), &y = tensor(a[1], "b");
+    if (x.dim() != 2 || y.dim() != 2) raise(PyExc_ValueError, "matrices are needed");
+    return PyBool_FromLong(shares_memory(x, y));
+  });
+}
+
 PyObject* py_bind(PyObject*, PyObject* args) {  // two error classes, five addresses
   PyObject *cls, *oom;
   unsigned long long p[5];
@@ -326,6 +355,7 @@ PyMethodDef methods[] = {
     {"quantize", (PyCFunction)(void*)py_quantize, METH_FASTCALL, nullptr},
     {"rmsnorm_quant", (PyCFunction)(void*)py_rmsnorm_quant, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void*)py_linear, METH_FASTCALL, nullptr},
+    {"shares_memory", (PyCFunction)(void*)py_shares_memory, METH_FASTCALL, nullptr},
     {"linear_swiglu", (PyCFunction)(void*)py_linear_swiglu, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -71,7 +71,8 @@ def rmsnorm_quant(x, weight, eps: float = 1e-6, residual=None, position=None):
 def linear(x, x_scale, w, w_scale, out_dtype=torch.bfloat16, out=None):
     """``x @ w.T`` of e4m3 matrices with their scales: x ``[M, K]``, w ``[N, K]`` -> ``[M, N]`` in bf16, fp16
     or fp32, summed in fp32. ``out``: a matrix of that shape to write, of any of the three types (``out_dtype`` is then not
-    read), its rows contiguous, that shares no memory with the inputs."""
+    read), its rows contiguous, that shares no memory with the inputs: one that does is refused, and so is one that only
+    meets an input's span without sharing a byte, where the two have rows of different pitch."""
     return (_native or _load()).linear(x, x_scale, w, w_scale, out_dtype, out)
 
 

@@ -5,7 +5,9 @@ import re
 from pathlib import Path
 
 import pytest
+import torch
 
+from ignite_xdna_b200 import fp8
 from test_fp8 import plan
 
 SM_SHARED, SYSTEM = 228 * 1024, 1024  # an SM's shared memory, and what the system takes of it per CTA
@@ -41,3 +43,40 @@ def test_fp8_kernels_read_nothing_as_read_only():
     text, parts = kernels("ixb_fp8.cuh")
     assert all("grid_dep_wait" in k for k in parts) and len(parts) == 4
     assert not re.search(r"\.nc\b|__ldg|__restrict__", text)
+
+
+# ---------------------------------------------------------------- arguments
+def places(t):
+    """The bytes that a matrix takes, as a set of addresses."""
+    size, row = t.element_size(), t.stride(0) * t.element_size()
+    return {t.data_ptr() + i * row + j for i in range(t.shape[0]) for j in range(t.shape[1] * size)}
+
+
+def test_what_shares_memory():
+    """Against the sets of bytes: exact where rows are equally far apart or one matrix has one row, never 'no' for matrices
+    that share a byte, never 'yes' for spans that do not meet."""
+    fp8._load()
+    shares = fp8._native.shares_memory
+    r = random.Random(3)
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    seen = [0, 0]
+    for _ in range(4000):
+        views = []
+        pitch = 4 * r.randint(1, 16)
+        for _ in range(2):
+            t = buf.view(r.choice((torch.uint8, torch.bfloat16, torch.float32)))
+            size = t.element_size()
+            step = (pitch if r.random() < 0.7 else 4 * r.randint(1, 16)) // size
+            rows, cols = r.randint(1, 6), r.randint(1, step)
+            views.append(t.as_strided((rows, cols), (step, 1), r.randint(0, 160) // size))
+        a, b = views
+        pa, pb = places(a), places(b)
+        got, true = shares(a, b), bool(pa & pb)
+        assert got or not true
+        if a.shape[0] == 1 or b.shape[0] == 1 or a.stride(0) * a.element_size() == b.stride(0) * b.element_size():
+            assert got == true, (a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype)
+            seen[true] += 1
+        if max(pa) < min(pb) or max(pb) < min(pa):
+            assert not got
+    assert min(seen) > 200
+    assert not shares(buf.view(64, 64)[:0], buf.view(64, 64))

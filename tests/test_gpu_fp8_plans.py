@@ -37,3 +37,35 @@ def test_launches_that_take_over_one_anothers_sms():
         settle()
         for g, e in zip(got, want[turn % 5:] + want[:turn % 5]):
             assert all(same_bits(a, b) for a, b in zip(g, e))
+
+
+# ---------------------------------------------------------------- out=
+def test_padded_out_over_an_input_is_refused_and_beside_it_is_not():
+    """Views of wider matrices: refused where a byte is shared with an operand or its scales, taken where the columns
+    of one matrix are divided between them."""
+    M, N, K = 40, 64, 512
+    x, xs = F.make(M, K, 1, 0, device="cuda")
+    w, ws = F.make(N, K, 128, 1, device="cuda")
+    want = fp8.linear(x, xs, w, ws)
+    buf = torch.zeros(64, 1024, dtype=torch.uint8, device="cuda")
+    buf[:M, :K] = x.view(torch.uint8)
+    wide_x = buf[:M, :K].view(fp8.E4M3)
+    before = buf.clone()
+    bf16 = buf.view(torch.bfloat16)
+    for rows, out in ((slice(0, M), bf16[:M, 224:288]), (slice(0, M), bf16[:M, 0:64]), (slice(0, 24), bf16[23:47, 255:319])):
+        with pytest.raises(ValueError, match="shares memory"):
+            fp8.linear(wide_x[rows], xs[rows], w, ws, out=out)
+    buf_w = torch.zeros(N, 1024, dtype=torch.uint8, device="cuda")
+    buf_w[:, 512:] = w.view(torch.uint8)
+    with pytest.raises(ValueError, match="shares memory"):
+        fp8.linear(x, xs, buf_w[:, 512:].view(fp8.E4M3), ws, out=buf_w.view(torch.bfloat16)[:M, 200:264])
+    buf_s = torch.zeros(M, 132, dtype=torch.uint8, device="cuda")
+    buf_s[:, 126:130] = xs.view(torch.uint8)
+    with pytest.raises(ValueError, match="shares memory"):
+        fp8.linear(x, buf_s[:, 126:130].view(fp8.E8M0), w, ws, out=buf_s.view(torch.bfloat16)[:, :64])
+    settle()
+    assert torch.equal(buf, before)
+    out = bf16[:M, 256:320]  # beside x in the same rows
+    assert fp8.linear(wide_x, xs, w, ws, out=out).data_ptr() == out.data_ptr()
+    settle()
+    assert torch.equal(out, want) and torch.equal(buf[:M, :K], before[:M, :K])
