@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -70,6 +71,8 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   if (t.layout() != at::kStrided) raise(PyExc_ValueError, "%s: a strided tensor is needed", name);
   if (t.requires_grad() && at::GradMode::is_enabled())
     raise(PyExc_ValueError, "%s requires grad: these operators have no backward pass (call them under torch.no_grad())", name);
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    raise(PyExc_ValueError, "%s has a forward-mode tangent, which these operators would drop: they have no derivative", name);
   return t;
 }
 

@@ -14,7 +14,7 @@ Matrices are two-dimensional, their rows contiguous, 16-byte aligned and a multi
 widths are multiples of 16. Calls are enqueued on the current stream of the tensors' device and return
 before the kernels finish; they can be captured into a CUDA graph. Without the compiled library or a
 GPU they raise: there is no fallback. They are for inference: under grad mode an input that requires grad is
-refused, for there is no backward pass.
+refused, for there is no backward pass, and so is one with a forward-mode tangent.
 """
 from __future__ import annotations
 

@@ -80,3 +80,18 @@ def test_what_shares_memory():
             assert not got
     assert min(seen) > 200
     assert not shares(buf.view(64, 64)[:0], buf.view(64, 64))
+
+
+def test_a_forward_mode_tangent_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x = torch.zeros(4, 256)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match="tangent"):
+            fp8.quantize(dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # forward mode goes on under no_grad
+            fp8.rmsnorm_quant(x, dual[0])
+        with pytest.raises(ValueError, match="CUDA"):  # refused for its device alone
+            fp8.quantize(fwd.unpack_dual(dual).primal)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8.quantize(x)
