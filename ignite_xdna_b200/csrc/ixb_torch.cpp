@@ -69,6 +69,7 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s: a tensor is needed, got %s", name, Py_TYPE(o)->tp_name);
   const at::Tensor& t = THPVariable_Unpack(o);
   if (t.layout() != at::kStrided) raise(PyExc_ValueError, "%s: a strided tensor is needed", name);
+  if (t.is_neg()) raise(PyExc_ValueError, "%s: its memory holds the negated values (call resolve_neg() first)", name);
   if (t.requires_grad() && at::GradMode::is_enabled())
     raise(PyExc_ValueError, "%s requires grad: these operators have no backward pass (call them under torch.no_grad())", name);
   if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())

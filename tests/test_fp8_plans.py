@@ -95,3 +95,14 @@ def test_a_forward_mode_tangent_is_refused():
             fp8.quantize(fwd.unpack_dual(dual).primal)
     with pytest.raises(ValueError, match="CUDA"):
         fp8.quantize(x)
+
+
+def test_a_view_of_negated_values_is_refused():
+    """Its memory holds the opposite of its values, and the kernels read memory."""
+    x = torch.ones(4, 256)
+    with pytest.raises(ValueError, match="negated"):
+        fp8.quantize(torch._neg_view(x))
+    with pytest.raises(ValueError, match="negated"):
+        fp8.quantize(torch.ones(4, 256, dtype=torch.complex64).conj().imag)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8.quantize(torch._neg_view(x).resolve_neg())
