@@ -7,6 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
+import fp8_model as F
 from ignite_xdna_b200 import fp8
 from test_fp8 import plan
 
@@ -106,3 +107,19 @@ def test_a_view_of_negated_values_is_refused():
         fp8.quantize(torch.ones(4, 256, dtype=torch.complex64).conj().imag)
     with pytest.raises(ValueError, match="CUDA"):
         fp8.quantize(torch._neg_view(x).resolve_neg())
+
+
+# ---------------------------------------------------------------- what the GPU tests reach
+@pytest.mark.parametrize("swiglu", [0, 1])
+def test_the_gpu_tests_shapes_reach_every_form(swiglu):
+    shapes = F.SWIGLU_FORMS if swiglu else F.LINEAR_FORMS
+    tested = {F.form(plan(*s, swiglu), swiglu) for s in shapes}
+    r = random.Random(9)
+    spread = lambda a, b: int(round(a * (b / a) ** r.random()))  # noqa: E731
+    missing = {}
+    for _ in range(10000):
+        s = (spread(1, 8192), 16 * spread(1, 1024) if swiglu else spread(1, 16384), 16 * spread(1, 1024))
+        missing.setdefault(F.form(plan(*s, swiglu), swiglu), s)
+    missing = {f: s for f, s in missing.items() if f not in tested}
+    assert not missing
+    assert len(tested) >= (20 if swiglu else 34)

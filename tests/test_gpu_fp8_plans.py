@@ -1,11 +1,13 @@
 """The fp8 products in every form that the planner picks, at a decoder's depths: chains of launches, scale images
 that follow one another, accuracy of the 32-bit sums."""
+import math
+
 import pytest
 import torch
 
 import fp8_model as F
 from ignite_xdna_b200 import fp8
-from test_gpu_fp8 import same_bits, settle
+from test_gpu_fp8 import check_product, check_swiglu, layer, mlp, same_bits, settle
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +71,79 @@ def test_padded_out_over_an_input_is_refused_and_beside_it_is_not():
     assert fp8.linear(wide_x, xs, w, ws, out=out).data_ptr() == out.data_ptr()
     settle()
     assert torch.equal(out, want) and torch.equal(buf[:M, :K], before[:M, :K])
+
+
+# ---------------------------------------------------------------- every form, at a decoder's depths
+def make(M, K, rows, seed):
+    """As fp8_model.make, on the GPU: normal values, blocks of different sizes."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    v = torch.randn(M, K, generator=g, dtype=F.F64, device="cuda")
+    size = torch.exp2(4 * (torch.rand(-(-M // rows), -(-K // F.BLOCK), generator=g, dtype=F.F64, device="cuda") - 0.5))
+    q, e = F.quantize(v * F.spread(size, rows, M, K), rows)
+    return q.float().to(fp8.E4M3), (e + 127).to(torch.uint8).view(fp8.E8M0)
+
+
+def sum_error(K):
+    """Ten times the documented error of the 32-bit sums, relative to the result's norm, for normal values: 1e-7 up to a depth of
+    4096, 2.6e-7 up to 16384, 3e-6 up to 65536. (Each of a chain's K / 32 matrix instructions may cut at 2^-23 of the running
+    sum: 1e-5 at 4096 if every one did and all the same way. Products held in 16 bits are 1e-3 off.)"""
+    return 1e-6 if K <= 4096 else 2.6e-6 if K <= 16384 else 3e-5
+
+
+@pytest.mark.parametrize("M,N,K", F.LINEAR_FORMS + [(60, 300, 65536)])
+def test_linear_in_every_form(M, N, K):
+    x, xs = make(M, K, 1, seed=M + K)
+    w, ws = make(N, K, 128, seed=N + K)
+    out = fp8.linear(x, xs, w, ws, out_dtype=torch.float32)
+    settle()
+    check_product(x, xs, w, ws, out)
+    ref = F.values(x, xs, 1) @ F.values(w, ws, 128).t()
+    assert (out.double() - ref).norm() <= sum_error(K) * ref.norm()
+    for dtype in (torch.bfloat16, torch.float16):  # the same sums, rounded once
+        assert torch.equal(fp8.linear(x, xs, w, ws, out_dtype=dtype), out.to(dtype))
+    settle()
+
+
+def check_codes(x, xs, g, gs, u, us, q, s):
+    """How many e4m3 values are not the rounded 64-bit result's. A product off by d times the products' norm turns a value whose
+    product is t times that norm with a probability of at most 32 d / t (twice the relative error over e4m3's step of at
+    least 2^-4 of the value); over normal products that is 32 d times 0.8 ln(1 / 32 d), 2.7e-4 for d = 1e-6, for gate
+    and for up. Products held in 16 bits turn percents."""
+    K = x.shape[1]
+    gate, up = F.product(x, xs, g, gs)[0], F.product(x, xs, u, us)[0]
+    want, e = F.quantize(gate * torch.sigmoid(gate) * up, 1)
+    same = F.exponent_of(s) == e
+    share = 1e-3 * sum_error(K) / 1e-6
+    assert (~same).sum() <= 1 + share * same.numel()
+    turned = (q.float().double() != want) & F.spread(same, 1, *q.shape)
+    assert turned.sum() <= 1 + share * q.numel()
+
+
+@pytest.mark.parametrize("M,N,K", F.SWIGLU_FORMS)
+def test_swiglu_in_every_form(M, N, K):
+    x, xs = make(M, K, 1, seed=M + K)
+    g, gs = make(N, K, 128, seed=N + K)
+    u, us = make(N, K, 128, seed=N + K + 1)
+    down = int(round(0.5 * math.log2(K)))  # gates of a few units
+    gs, us = ((t.view(torch.uint8) - down).view(fp8.E8M0) for t in (gs, us))
+    q, s = fp8.linear_swiglu(x, xs, g, gs, u, us)
+    settle()
+    check_swiglu(x, xs, g, gs, u, us, q, s)
+    check_codes(x, xs, g, gs, u, us, q, s)
+
+
+@pytest.mark.parametrize("tokens", [1, 100, 777])
+def test_an_mlp_against_its_64_bit_chain(tokens):
+    """Norm, gate/up and down against the chain in 64 bits on the same weights without any rounding of activations. An e4m3
+    value is off by 2.7 % of itself in the mean square (half a step over its value is 2^-4 / m for a fraction m in [1, 2),
+    uniform below that): that much in gate and in up from the norm's values, together 4.5 % of gate/up's result with silu's
+    slope of up to 1.1 beside its value's, 2.7 % more from its own rounding: 5.3 % of the output's norm. Twice that is the limit."""
+    weights, x, r, nw = layer(tokens, 4096, 11008, seed=tokens)
+    (g, gs), (u, us), (d, ds) = weights
+    out, h, _ = mlp(weights, x, r, nw)
+    settle()
+    h64, y = F.norm(x, r, nw, 1e-6)
+    gate, up = (y @ F.values(t, ts, 128).t() for t, ts in ((g, gs), (u, us)))
+    ref = (gate * torch.sigmoid(gate) * up) @ F.values(d, ds, 128).t()
+    assert torch.equal(h, (x.float() + r.float()).bfloat16())
+    assert (out.double() - ref).norm() <= 0.106 * ref.norm()
