@@ -313,7 +313,9 @@ int ixb_fp8_quantize(const void* x, int type, int64_t ldx, int M, int K, int blo
  * in fp32, quantised to e4m3 with scales as above, or, with scale NULL, to int8 at a power-of-two
  * position in [-64, 64]: q = clamp(rne(y * 2^position), -128, 127), the activations of ixb_w4a8_gemm,
  * ixb_w4a8_gemv and ixb_i8gemm_srs. residual and h may both be NULL (y from x alone); h may be x or
- * residual itself. weight [K] has the type of x or fp32; K at most 32768. */
+ * residual itself. weight [K] has the type of x or fp32; K at most 32768. h * weight has to stay in fp32's
+ * range. A row with a NaN becomes NaN in e4m3 and 0 in int8, which has no NaN; in a row with an infinity the finite
+ * values become 0 and the infinity NaN, or 0 in int8. h keeps what is not finite. */
 int ixb_rmsnorm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, int type,
                       int weight_type, int M, int K, float eps, int position, void* h, int64_t ldh, uint8_t* q, int64_t ldq,
                       uint8_t* scale, int64_t lds, void* stream);

@@ -147,3 +147,24 @@ def test_an_mlp_against_its_64_bit_chain(tokens):
     ref = (gate * torch.sigmoid(gate) * up) @ F.values(d, ds, 128).t()
     assert torch.equal(h, (x.float() + r.float()).bfloat16())
     assert (out.double() - ref).norm() <= 0.106 * ref.norm()
+
+
+# ---------------------------------------------------------------- int8 norm, values that are not finite
+@pytest.mark.parametrize("M", [4, 400])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_norm_to_int8_of_what_is_not_finite(M, dtype):
+    """A NaN makes its row's root NaN, and NaN has no int8: the row is 0. An infinity makes the root 0, so the finite values
+    are 0, and 0 * inf = NaN is 0 as well. Other rows are as they would be."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(M, 512, generator=g).to(dtype).cuda()
+    w = torch.randn(512, generator=g).to(dtype).cuda()
+    want, _, _ = fp8.rmsnorm_quant(x, w, position=4)
+    x[0] = 0
+    x[1, 7] = math.nan
+    x[2, 9] = math.inf
+    x[3, 0], x[3, 1] = -math.inf, math.nan
+    q, s, h = fp8.rmsnorm_quant(x, w, position=4)
+    qr, _, h = fp8.rmsnorm_quant(x, w, position=4, residual=torch.zeros_like(x))
+    settle()
+    assert s is None and (q[:4] == 0).all() and torch.equal(q[4:], want[4:]) and torch.equal(q, qr)
+    assert torch.equal(torch.nan_to_num(h, nan=7.0), torch.nan_to_num(x, nan=7.0))  # the residual stream keeps them
