@@ -74,7 +74,8 @@ __device__ __forceinline__ uint32_t w4_hi16(uint32_t x) { return x & 0xF0F0F0F0u
 // launch at once, so in a chain of GEMVs (a decode step's layers) the next one's CTAs ask for
 // their weight ranges in the L2 (a bulk prefetch: a hint, which reads nothing they use) while this
 // one streams; every load whose value a CTA uses comes after it waits for the previous kernel
-// (griddepcontrol.wait).
+// (griddepcontrol.wait). The activations, which that kernel may still write when this one starts, are
+// read with plain loads; only the weight image and its tables are read-only data.
 constexpr int kGemvWarps = 8;
 constexpr int kGemvThreads = 32 * kGemvWarps;
 constexpr int kGemvBatch = 8;           // 16-byte loads per lane in flight
@@ -92,8 +93,8 @@ __device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
 // once serve both. Longer columns take one column per warp and batches of eight loads.
 template <int CPW>
 __global__ void __launch_bounds__(kGemvThreads, 4)
-    w4a8_gemv_kernel(const int8_t* __restrict__ a, const uint8_t* __restrict__ wq, const uint8_t* __restrict__ eg,
-                     const int32_t* __restrict__ shift, int8_t* __restrict__ out, int N, int K) {
+    w4a8_gemv_kernel(const int8_t* a, const uint8_t* __restrict__ wq, const uint8_t* __restrict__ eg,
+                     const int32_t* __restrict__ shift, int8_t* out, int N, int K) {
   constexpr int B = kGemvBatch / CPW;  // loads per column per batch
   const int n0 = blockIdx.x * kGemvWarps * CPW, warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -126,8 +127,8 @@ __global__ void __launch_bounds__(kGemvThreads, 4)
     for (int j = 0; j < B; ++j) {
       const int k = k0 + j * 1024;
       if (k < K) {
-        const int4 a0 = __ldg(reinterpret_cast<const int4*>(a + k));
-        const int4 a1 = __ldg(reinterpret_cast<const int4*>(a + k) + 1);
+        const int4 a0 = reinterpret_cast<const int4*>(a + k)[0];
+        const int4 a1 = reinterpret_cast<const int4*>(a + k)[1];
 #pragma unroll
         for (int c = 0; c < CPW; ++c) {
           if (!ok[c]) continue;

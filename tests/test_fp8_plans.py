@@ -123,3 +123,11 @@ def test_the_gpu_tests_shapes_reach_every_form(swiglu):
     missing = {f: s for f, s in missing.items() if f not in tested}
     assert not missing
     assert len(tested) >= (20 if swiglu else 34)
+
+
+def test_the_gemv_reads_its_activations_as_what_another_kernel_writes():
+    """It starts while the kernel before, a norm or another GEMV, may still write them."""
+    _, parts = kernels("ixb_w4a8.cuh")
+    gemv = next(k for k in parts if "w4a8_gemv_kernel(" in k)
+    assert "grid_dep_launch" in gemv and "const int8_t* a," in gemv and "int8_t* out," in gemv
+    assert not re.search(r"__ldg\((reinterpret_cast<const int4\*>\()?a\b", gemv)

@@ -168,3 +168,61 @@ def test_norm_to_int8_of_what_is_not_finite(M, dtype):
     settle()
     assert s is None and (q[:4] == 0).all() and torch.equal(q[4:], want[4:]) and torch.equal(q, qr)
     assert torch.equal(torch.nan_to_num(h, nan=7.0), torch.nan_to_num(x, nan=7.0))  # the residual stream keeps them
+
+
+# ---------------------------------------------------------------- chains of int8 products
+def test_norms_and_gemvs_in_turn_on_the_same_buffers():
+    """Two activation buffers written in turn by an int8 norm and by the GEMVs behind it, launched without a wait and in a graph: each reads
+    what the kernel before it wrote, not what lay there a step earlier."""
+    import ctypes as C
+
+    import numpy as np
+
+    import ixb_oracle as O
+    from ignite_xdna_b200 import _lib as L
+    K, steps, lib = 1024, 12, L.load()
+    rng = np.random.default_rng(4)
+    nw = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    layers = []
+    for _ in range(3):
+        w4 = O.pack_int4(rng.integers(-8, 8, size=(K, K), dtype=np.int8))
+        gpos = (5 + rng.integers(0, 4, size=(K // 128, K))).astype(np.int8)
+        shift = rng.integers(9, 12, size=K).astype(np.int32)
+        nbytes = C.c_uint64()
+        L.check(lib.ixb_w4a8_image_bytes(K, K, C.byref(nbytes)))
+        img = torch.empty(nbytes.value, dtype=torch.uint8, device="cuda")
+        dw, dg, ds = (torch.from_numpy(v).cuda() for v in (w4, gpos, shift))
+        L.check(lib.ixb_w4a8_prepare(dw.data_ptr(), dg.data_ptr(), K, K, img.data_ptr(), None))
+        layers.append((img, ds, w4, gpos, shift))
+    torch.cuda.synchronize()
+    xs = [torch.randn(1, K, device="cuda").bfloat16() for _ in range(steps)]
+    bufs = [torch.zeros(1, K, dtype=torch.int8, device="cuda") for _ in range(2)]
+    kept = torch.zeros(steps, K, dtype=torch.int8, device="cuda")
+
+    def chain(stream):
+        for i, x in enumerate(xs):
+            L.check(lib.ixb_rmsnorm_quant(x.data_ptr(), K, None, 0, nw.data_ptr(), L.BF16, L.BF16, 1, K, 1e-6, 5, None, 0,
+                                          bufs[0].data_ptr(), K, None, 0, stream))
+            for j, (img, ds, *_) in enumerate(layers):
+                to = kept[i] if j == 2 else bufs[1 - j % 2]
+                L.check(lib.ixb_w4a8_gemv(bufs[j % 2].data_ptr(), img.data_ptr(), ds.data_ptr(), to.data_ptr(), K, K, stream))
+
+    want = []
+    for x in xs:
+        a = fp8.rmsnorm_quant(x, nw, position=5)[0].cpu().numpy()
+        for _, _, w4, gpos, shift in layers:
+            a = O.w4a8_srs(a, w4, gpos, shift)
+        want.append(a[0])
+    want = torch.from_numpy(np.stack(want))
+    chain(torch.cuda.current_stream().cuda_stream)
+    settle()
+    assert torch.equal(kept.cpu(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(torch.cuda.current_stream().cuda_stream)
+    for _ in range(5):
+        kept.zero_()
+        graph.replay()
+        settle()
+        assert torch.equal(kept.cpu(), want)
+    assert len(set(map(bytes, want.numpy()))) == steps and (want != 0).any()
