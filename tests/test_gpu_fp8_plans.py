@@ -226,3 +226,90 @@ def test_norms_and_gemvs_in_turn_on_the_same_buffers():
         settle()
         assert torch.equal(kept.cpu(), want)
     assert len(set(map(bytes, want.numpy()))) == steps and (want != 0).any()
+
+
+# ---------------------------------------------------------------- two streams
+def test_clusters_of_several_launches_on_two_streams():
+    """Products whose CTAs wait for one another, in both forms, at once on three streams: gate/up with the widest few-token tiles, a small
+    product that leaves shared memory free, a pair product. Every launch gets its TMEM, and the same bits as alone."""
+    def problem(M, N, K, swiglu):
+        x, xs = make(M, K, 1, M + K)
+        w, ws = make(N, K, 128, N)
+        if not swiglu:
+            return lambda: [fp8.linear(x, xs, w, ws)]
+        u, us = make(N, K, 128, N + 1)
+        return lambda: list(fp8.linear_swiglu(x, xs, w, ws, u, us))
+
+    calls = [problem(120, 3664, 12880, True), problem(32, 4096, 2048, False), problem(700, 2048, 512, False)]
+    want = [c() for c in calls]
+    settle()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for turn in range(6):
+        got = [[] for _ in calls]
+        for _ in range(10):
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    got[i].append(calls[(i + turn) % 3]())
+        settle()
+        for i, outs in enumerate(got):
+            assert all(same_bits(a, b) for o in outs for a, b in zip(o, want[(i + turn) % 3]))
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+def rows_in_turn(M, K, dtype, seed):
+    """[M, K] of 4099 different rows, so that neighbouring tiles differ and no row has the same place in its tile twice in turn."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    some = torch.randn(4099, K, generator=g, device="cuda").to(dtype)
+    return some[torch.arange(M, device="cuda") % 4099]
+
+
+def test_row_operators_past_32_bit_offsets():
+    """More than 2^31 values: every row as the same row of a small call."""
+    M, K = 540_000, 4096
+    x = rows_in_turn(M, K, torch.bfloat16, 1)
+    nw = torch.randn(K, device="cuda").bfloat16()
+    small = x[:4099].clone()
+
+    def check(big, want):
+        settle()
+        for b, w in zip(big, want):
+            b, w = b.view(torch.uint8), w.view(torch.uint8)
+            for at in range(0, M, 4099):
+                part = b[at:at + 4099]
+                assert torch.equal(part, w[:len(part)]), at
+
+    want = fp8.quantize(small)
+    check(fp8.quantize(x), want)
+    want = fp8.rmsnorm_quant(small, nw, residual=small)
+    check(fp8.rmsnorm_quant(x, nw, residual=x), want)
+    del x
+    x = rows_in_turn(4_200_000, 528, torch.bfloat16, 2)
+    q, s = fp8.quantize(x, block_rows=128)
+    settle()
+    last = 32_812 * 128  # the last whole blocks and the short one behind them
+    for at in (0, last - 4096, 4_200_000 // 128 * 128 - 256):
+        qp, sp = fp8.quantize(x[at:at + 4096], block_rows=128)
+        settle()
+        assert same_bits(q[at:at + 4096], qp) and same_bits(s[at // 128:at // 128 + len(sp)], sp)
+
+
+@pytest.mark.parametrize("M,N,K", [(135_000, 16400, 128), (1_100_000, 144, 2064)])
+def test_products_past_32_bit_offsets(M, N, K):
+    """More than 2^31 outputs, and more than 2^31 bytes of x: the rows at both ends against the 64-bit form."""
+    x, xs = fp8.quantize(rows_in_turn(M, K, torch.bfloat16, 3))
+    w, ws = make(N, K, 128, 4)
+    out = fp8.linear(x, xs, w, ws)
+    settle()
+    ends = (slice(0, 300), slice(M // 2, M // 2 + 300), slice(M - 300, M))
+    for rows in ends:
+        check_product(x[rows], xs[rows], w, ws, out[rows])
+    del out
+    N = N // 16 * 16
+    u, us = make(N, K, 128, 5)
+    w, ws = w[:N], ws[:-(-N // 128)]
+    down = int(round(0.5 * math.log2(K)))
+    ws, us = ((t.view(torch.uint8) - down).view(fp8.E8M0) for t in (ws, us))
+    q, s = fp8.linear_swiglu(x, xs, w, ws, u, us)
+    settle()
+    for rows in ends:
+        check_swiglu(x[rows], xs[rows], w, ws, u, us, q[rows], s[rows])
