@@ -205,7 +205,8 @@ __device__ __forceinline__ uint2 round8(float (&f)[8], float m) {
 // ---------------------------------------------------------------- quantise
 // The pointers carry no __restrict__: the kernel before may still be writing x when one of these starts, so its
 // loads must not become loads of read-only data.
-// Rows in blocks of 1 x 128: 16 lanes per block, eight values per lane. Bound by HBM.
+// Rows in blocks of 1 x 128: 16 lanes per block, eight values per lane. Bound by HBM (11008 x 4096: 25.3 us in
+// bf16, 5.3 TB/s, 35.5 in fp32, 6.4).
 constexpr int kQThreads = 256;
 constexpr int kQUnroll = 4;  // blocks per half-warp, so four 16-byte loads per lane are in flight
 template <typename T>
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kQThreads)
 // A weight's 128 x 128 blocks: a CTA per block, V vectors of eight per thread held in registers, as they lie
 // in memory, between the maximum and the rounding, so the weight is read once. Bound by HBM: four
 // CTAs' loads are in flight on an SM. (Kept unpacked, the values spill or leave room for two CTAs:
-// 38 and 31 us for 11008 x 4096 bf16 instead of 22.6, 5.97 TB/s.)
+// 38 and 31 us for 11008 x 4096 bf16 instead of 21.5, 6.3 TB/s; fp32, with two, 34.6 us, 6.5 TB/s.)
 constexpr int kTileThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2)
@@ -329,7 +330,10 @@ struct NormParams {
 // between the sum of squares and the output, so the row is read once. With many rows HBM bounds it,
 // and the next row's loads (without a residual the next two rows') are issued before this row's barrier, so
 // that they are in flight while it is reduced and rounded, and the weight stays in registers (V up to
-// 2 and 16-bit values: more would spill). With few rows: one load, one barrier and one store.
+// 2 and 16-bit values: more would spill): 8192 x 4096 bf16 with a residual 38.5 us (6.1 TB/s), without one 28.0 us
+// (3.6 TB/s, bound by instructions), fp32 70 us (6.2 TB/s). V 8, for rows above 16384 values, spills even so (80 to
+// 352 bytes a thread): 512 x 32768 with a residual 33.4 us in bf16 (3.5 TB/s), 65.3 in fp32 (3.3). With few rows:
+// one load, one barrier and one store.
 template <typename T, typename W, int V>
 __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const __grid_constant__ NormParams p) {
   constexpr bool kAhead = V <= 2 && sizeof(T) == 2;
@@ -465,12 +469,18 @@ __global__ void __launch_bounds__(V <= 2 ? 1024 : 512) norm_quant_kernel(const _
 // eight CTAs shares a tile along K and adds its 32-bit parts in rank order over distributed shared
 // memory; shared memory and registers leave room for two CTAs per SM, so the next kernel's start
 // overlaps this one's end. HBM bounds it (the weights are read once), with ~3 us of start and end:
-// 1 x 4096 x 4096 5.8 us, 23 x 4096 x 11008 11.9 us (3.8 TB/s), 8 x 11008 x 4096 gate/up 18 us (5 TB/s). (Asking the weights into L2 before waiting for the previous kernel, as the
-// W4A8 GEMV does, gained nothing: 18.4 us without and 20.0 with it for 8 x 11008 x 4096 gate/up.) Many
-// tokens (CG 2): persistent pairs of CTAs, tiles of 256 weight rows x 224 tokens with two accumulators
-// (or 512 rows and one, where that is one round). The tensor cores bound it, and in a long run the
-// board's 1000 W: 8192 x 11008 x 4096 takes 256 us (2.9 PFLOP/s) in a burst and 301 us at the ~1.05 GHz
-// that the cap leaves, where the MMAs alone would take 300.
+// 1 x 4096 x 4096 5.7 us, 23 x 4096 x 11008 11.9 us (3.8 TB/s), 8 x 11008 x 4096 gate/up 18.5 us (4.9 TB/s).
+// (Asking the weights into L2 before waiting for the previous kernel, as the W4A8 GEMV does, made the last of
+// these 9 % slower and the others no faster.)
+// Many tokens (CG 2): persistent pairs of CTAs, tiles of 256 weight rows x 224 tokens with two accumulators
+// (or 512 rows and one, where that is one round). The tensor cores bound it, and in a long run the board's
+// 1000 W: 8192 x 11008 x 4096 takes 262 us (2.8 PFLOP/s) in a burst and 318 us in a long run, at ~1.05 GHz, where
+// the MMAs alone would take 300. A prompt chunk is bound by its operands' arrival and by what of the MMAs does
+// not overlap it: 512 x 4096 x 11008 takes 0.229 us for a K-block of 128 tokens, 0.182 without the MMAs and 0.146
+// without the loads.
+// The tensor cores cut a running sum where an fp32 adder rounds, about once per K-block: 2e-8 to 3e-8 of the
+// result's norm for each K-block of a chain. Taken as it is: with K = 65536 in one chain it is 1.7e-5, far below
+// the rounding of a 16-bit or e4m3 output, and shorter chains would drain each accumulator several times per tile.
 constexpr int kFp8Epi = 8;                               // epilogue warps, two groups of four
 constexpr int kFp8Threads = 32 * (kFp8Epi + 3);          // + TMA producer, MMA issuer, scale gatherer
 constexpr int kFp8MaxStages = 12;
@@ -827,7 +837,7 @@ __device__ __forceinline__ void swiglu_columns(const Fp8Params& p, uint32_t (&ga
 
 // Tiles go through n in groups of p.n_group and through all m within a group, n first: the tiles in work at
 // one time then form a near-square, and what they read (a group's weights, a few rows of x) is read
-// from L2 by as few as can be (8192 x 11008 x 4096: 270 us, through all of n first 279).
+// from L2 by as few as can be (8192 x 11008 x 4096 takes 3 % longer through all of n first).
 __device__ __forceinline__ void tile_at(const Fp8Params& p, int t, int& mt, int& nt) {
   const int per = p.n_group * p.m_tiles, g = t / per, r = t - g * per;
   const int size = min(p.n_group, p.n_tiles - g * p.n_group);
@@ -912,7 +922,7 @@ __global__ void __launch_bounds__(kFp8Threads, CG == 1 ? 2 : 1) fp8_gemm_kernel(
     // ------------------------------------------------------------ TMA producer
     // This warp's and the MMA warp's loops run in all lanes and one elected lane issues, so addresses and
     // descriptors stay in uniform registers (with the loops inside `if (lane == 0)` 8192 x 11008 x 4096
-    // took 372 us instead of 318, at that time).
+    // takes 17 % longer).
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
